@@ -26,6 +26,9 @@ SOURCES = [
     CSRC / "gsp_prefill_mfma.hip",
     CSRC / "gsp_pool_ops.hip",
     CSRC / "gsp_matmul.hip",
+    CSRC / "gsp_matmul_fp8.hip",
+    CSRC / "gsp_row_ops.hip",
+    CSRC / "gsp_mrope.hip",
     CSRC / "gsp_noalloc.hip",
     CSRC / "gsp_runtime.cpp",
     CSRC / "gsp_step_plan.cpp",

@@ -158,6 +158,83 @@ struct RopeWriteArgs {
 
 hipError_t launch_rope_write(int kv_f16, const RopeWriteArgs& a, hipStream_t stream);
 
+// Rotation by positions of several axes and Store (gsp_mrope.hip).
+constexpr int kMropeMaxAxes = 4;
+struct MropeWriteArgs {
+    void* k_pool;
+    void* v_pool;
+    int64_t block_stride;
+    int64_t layer_offset;
+    int64_t head_stride;
+    int64_t v_block_stride;
+    int64_t v_layer_offset;
+    int64_t v_head_stride;
+    const int32_t* positions;  // [n_axes][n]
+    const int32_t* block_ids;  // [n]; -1: no slot, K and V not stored
+    const int32_t* slots;      // [n]
+    const float* q;            // rows of q_stride floats, n_heads x head_dim in each
+    const float* k;            // rows of k_stride
+    const float* v;            // rows of v_stride
+    float* q_out;              // [n][n_heads][head_dim]; may be q where q's rows are as dense
+    int64_t q_stride;
+    int64_t k_stride;
+    int64_t v_stride;
+    const double* freq;        // as in RopeWriteArgs
+    double log2_base;
+    int32_t n;
+    int32_t n_heads;
+    int32_t n_kv;
+    int32_t head_dim;
+    int32_t v_head_dim;
+    int32_t style;
+    int32_t rope_dim;
+    float mscale;
+    int32_t n_axes;
+    int32_t interleaved;               // GSP_MROPE_INTERLEAVED
+    int32_t sections[kMropeMaxAxes];   // pairs of each axis
+};
+hipError_t launch_mrope_write(int kv_f16, const MropeWriteArgs& a, hipStream_t stream);
+
+// Row operators (gsp_row_ops.hip).
+struct RmsNormArgs {
+    const float* x;         // [rows][dim]
+    const float* residual;  // [rows][dim] or null
+    const float* weight;    // [dim]
+    float* sum;             // [rows][dim] x + residual, or null
+    float* y;               // [rows][dim] or null
+    uint8_t* codes;         // [rows][dim] e4m3, or null
+    float* scale;           // [rows] with codes
+    float eps;
+    int32_t rows;
+    int32_t dim;
+};
+hipError_t launch_rms_norm(const RmsNormArgs& a, hipStream_t stream);
+
+struct QuantizeArgs {
+    const float* a;   // rows of `stride` floats, dim of them used
+    const float* b;   // null: codes of a; else of silu(a) * b
+    uint8_t* codes;   // [rows][dim]
+    float* scale;     // [rows]
+    int64_t stride;
+    int32_t rows;
+    int32_t dim;
+};
+hipError_t launch_quantize_fp8(const QuantizeArgs& a, hipStream_t stream);
+
+// Projections of e4m3 activations by 4-bit weights (gsp_matmul_fp8.hip).
+struct MatmulFp8Args {
+    const void* w;         // out_dim rows of row_bytes
+    const uint8_t* x;      // [batch][in_dim] e4m3
+    const float* x_scale;  // [batch]
+    float* y;              // [batch][out_dim]
+    int64_t row_bytes;
+    int32_t in_dim;        // a multiple of 64 (Q4_K: of 256)
+    int32_t out_dim;
+    int32_t batch;
+};
+int64_t matmul_fp8_row_bytes(int32_t w_type, int32_t in_dim);
+hipError_t launch_matmul_fp8(int32_t w_type, const MatmulFp8Args& a, hipStream_t stream);
+
 // Projection GEMM (gsp_matmul.hip): y[b][o] = sum_i W[o][i] x[b][i].
 constexpr int kWeightF32 = 0;   // GGUF type ids
 constexpr int kWeightQ8_0 = 8;

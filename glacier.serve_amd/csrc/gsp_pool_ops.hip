@@ -2,6 +2,7 @@
 // the same scatter with the rotary embedding applied on the way, and the
 // copy-on-write page copy.  All are small HBM-bound copies.
 #include "gsp_internal.h"
+#include "gsp_rope.h"
 #include "../../include/glacier_paged.h"
 
 namespace gsp {
@@ -34,26 +35,6 @@ __global__ __launch_bounds__(128) void write_tokens_kernel(WriteTokensArgs a) {
     if (e1 < a.v_head_dim) vd[e1] = static_cast<KT>(v1);
     for (int e = e0 + 256; e < a.head_dim; e += 128) kd[e] = static_cast<KT>(ks[e]);
     for (int e = e0 + 256; e < a.v_head_dim; e += 128) vd[e] = static_cast<KT>(vs[e]);
-}
-
-// Cosine and sine of pair j's angle at position `pos`, times the rotation's
-// scale (shared by both RoPE kernels).  The angle, pos times the pair's rate
-// (the table's, or freq_base^(-2j/rope_dim)), is formed and reduced to
-// [-pi, pi] in fp64, so it stays exact at long positions; cosine and sine are
-// fp32.  A scale of 1 leaves them exact.
-__device__ inline void rope_angle(const RopeWriteArgs& a, double pos, int j, float* c, float* s) {
-    const double rate = a.freq ? a.freq[j] : exp2(-(2.0 * j / a.rope_dim) * a.log2_base);
-    const double ang = pos * rate;
-    const double r = ang - 6.283185307179586 * rint(ang * 0.15915494309189535);
-    float sn, cn;
-    sincosf((float)r, &sn, &cn);
-    *c = cn * a.mscale;
-    *s = sn * a.mscale;
-}
-
-__device__ inline void rope_turn(float x0, float x1, float c, float s, float* y0, float* y1) {
-    *y0 = x0 * c - x1 * s;
-    *y1 = x0 * s + x1 * c;
 }
 
 // QuantKernels.RoPE then PagedBlockPool.Store for n tokens
@@ -112,17 +93,6 @@ __global__ __launch_bounds__(256) void rope_write_kernel(RopeWriteArgs a) {
         const int e = idx - hk * dv;
         static_cast<KT*>(a.v_pool)[vdst + (int64_t)hk * a.v_head_stride + e] =
             static_cast<KT>(a.v[((int64_t)i * a.n_kv + hk) * dv + e]);
-    }
-}
-
-template <typename KT>
-__device__ inline void store4(KT* p, const float4& x) {
-    if constexpr (sizeof(KT) == 4) {
-        *reinterpret_cast<float4*>(p) = x;
-    } else {
-        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-        h4 h = {(_Float16)x.x, (_Float16)x.y, (_Float16)x.z, (_Float16)x.w};
-        *reinterpret_cast<h4*>(p) = h;
     }
 }
 

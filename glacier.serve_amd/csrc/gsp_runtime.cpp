@@ -890,6 +890,37 @@ int check_write_step(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, const float* k
     return set_device(ctx);
 }
 
+// The axes of a rotation against the head's pairs.
+int check_mrope_axes(const gsp_mrope_spec& m, int32_t half) {
+    if (m.n_axes < 1 || m.n_axes > GSP_MROPE_MAX_AXES)
+        return gsp::fail(GSP_E_INVALID_ARG, "M-RoPE takes 1 to %d axes (got %d)", GSP_MROPE_MAX_AXES, m.n_axes);
+    if (m.layout != GSP_MROPE_SECTIONS && m.layout != GSP_MROPE_INTERLEAVED)
+        return gsp::fail(GSP_E_INVALID_ARG, "unknown M-RoPE layout %d", m.layout);
+    int64_t pairs = 0;
+    for (int32_t i = 0; i < m.n_axes; ++i) {
+        if (m.sections[i] < 0) return gsp::fail(GSP_E_INVALID_ARG, "M-RoPE section %d is negative", i);
+        pairs += m.sections[i];
+        if (m.layout == GSP_MROPE_INTERLEAVED && i > 0 && m.sections[i] > 0 &&
+            (int64_t)m.n_axes * (m.sections[i] - 1) + i >= half)
+            return gsp::fail(GSP_E_INVALID_ARG, "axis %d does not find its %d pairs among the head's %d", i, m.sections[i], half);
+    }
+    if (pairs != half)
+        return gsp::fail(GSP_E_INVALID_ARG, "the M-RoPE sections hold %lld pairs, the rotation %d", (long long)pairs, half);
+    return GSP_OK;
+}
+
+// Bytes of device memory that a call reads or writes.
+struct Span {
+    const void* p;
+    int64_t bytes;
+};
+bool overlap(const Span& a, const Span& b) {
+    if (!a.p || !b.p) return false;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+}
+bool is_aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
 }  // namespace
 
 extern "C" {
@@ -933,6 +964,197 @@ int gsp_rope_write_step(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, int32_t n_h
                         float* q_dev, const float* k_dev, const float* v_dev) {
     const gsp_rope_spec spec = plain_rope(freq_base, style);
     return gsp_rope_write_step_ex(ctx, pool, layer, n_heads, &spec, q_dev, k_dev, v_dev);
+}
+
+int gsp_mrope_write_step(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, int32_t n_heads, const gsp_mrope_spec* spec,
+                         const int32_t* positions_dev, const float* q_dev, int64_t q_stride, float* q_out_dev,
+                         const float* k_dev, int64_t k_stride, const float* v_dev, int64_t v_stride) try {
+    gsp::clear_error();
+    int rc = check_write_step(ctx, pool, layer, k_dev, v_dev);
+    if (rc) return rc;
+    if (!spec) return gsp::fail(GSP_E_INVALID_ARG, "M-RoPE spec is NULL");
+    RopeSetup r;
+    rc = check_rope(nullptr, pool, n_heads, &spec->rope, q_dev, &r);
+    if (!rc) rc = check_mrope_axes(*spec, r.rope_dim / 2);
+    if (rc) return rc;
+    const gsp_pool_desc& d = pool->desc;
+    const int32_t n = ctx->info.total_q;
+    const int64_t wide = (int64_t)n_heads * d.head_dim, wide_k = (int64_t)d.heads_kv * d.head_dim,
+                  wide_v = (int64_t)d.heads_kv * d.v_head_dim;
+    if (q_stride == 0) q_stride = wide;
+    if (k_stride == 0) k_stride = wide_k;
+    if (v_stride == 0) v_stride = wide_v;
+    const int64_t most = INT64_MAX / 8 / std::max(n, 1);
+    if (q_stride < wide || k_stride < wide_k || v_stride < wide_v || std::max({q_stride, k_stride, v_stride}) > most)
+        return gsp::fail(GSP_E_INVALID_ARG, "row strides (%lld, %lld, %lld) do not fit rows of %lld, %lld and %lld floats",
+                         (long long)q_stride, (long long)k_stride, (long long)v_stride, (long long)wide,
+                         (long long)wide_k, (long long)wide_v);
+    if (n == 0) return GSP_OK;
+    if (!positions_dev || (n_heads > 0 && !q_out_dev)) return gsp::fail(GSP_E_INVALID_ARG, "positions/q_out is NULL");
+    const auto span = [n](const void* p, int64_t stride, int64_t width) {
+        return Span{p, ((int64_t)(n - 1) * stride + width) * 4};
+    };
+    const Span q = span(q_dev, q_stride, wide), out = span(q_out_dev, wide, wide);
+    const Span rest[] = {span(k_dev, k_stride, wide_k), span(v_dev, v_stride, wide_v),
+                         Span{positions_dev, (int64_t)spec->n_axes * n * 4}};
+    if (!is_aligned(positions_dev, 4) || !is_aligned(q_dev, 4) || !is_aligned(q_out_dev, 4) || !is_aligned(k_dev, 4) ||
+        !is_aligned(v_dev, 4))
+        return gsp::fail(GSP_E_INVALID_ARG, "positions, q, k and v must be 4-byte aligned");
+    if (n_heads > 0) {
+        bool clash = overlap(out, q) && !(q_out_dev == q_dev && q_stride == wide);
+        for (const Span& s : rest) clash = clash || overlap(out, s);
+        if (clash) return gsp::fail(GSP_E_INVALID_ARG, "q_out overlaps an input (it may be q itself where q's rows are dense)");
+    }
+    bool cap = false;
+    rc = step_begin(ctx, &cap);
+    if (!rc) rc = check_rope(ctx, pool, n_heads, &spec->rope, q_dev, &r);
+    if (rc) return rc;
+    const int32_t* wr = ctx->d_step + ctx->off_wr;
+    gsp::MropeWriteArgs a{};
+    a.k_pool = pool->k;
+    a.v_pool = pool->v;
+    a.block_stride = pool->block_stride_k;
+    a.layer_offset = (int64_t)layer * pool->layer_stride_k;
+    a.head_stride = pool->head_stride_k;
+    a.v_block_stride = pool->block_stride_v;
+    a.v_layer_offset = (int64_t)layer * pool->layer_stride_v;
+    a.v_head_stride = pool->head_stride_v;
+    a.positions = positions_dev;
+    a.block_ids = wr + n;
+    a.slots = wr + 2 * (size_t)n;
+    a.q = q_dev;
+    a.k = k_dev;
+    a.v = v_dev;
+    a.q_out = q_out_dev;
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.freq = r.freq;
+    a.log2_base = r.log2_base;
+    a.n = n;
+    a.n_heads = n_heads;
+    a.n_kv = d.heads_kv;
+    a.head_dim = d.head_dim;
+    a.v_head_dim = d.v_head_dim;
+    a.style = r.style;
+    a.rope_dim = r.rope_dim;
+    a.mscale = r.mscale;
+    a.n_axes = spec->n_axes;
+    a.interleaved = spec->layout == GSP_MROPE_INTERLEAVED;
+    for (int32_t i = 0; i < spec->n_axes; ++i) a.sections[i] = spec->sections[i];
+    rc = check_hip(gsp::launch_mrope_write(d.kv_dtype == GSP_KV_F16, a, ctx->stream), "mrope_write launch");
+    const int rd = step_done(ctx, cap);
+    return rc ? rc : rd;
+} catch (const std::bad_alloc&) {
+    return gsp::fail(GSP_E_OOM, "host memory ran out");
+}
+
+int gsp_rms_norm(gsp_ctx* ctx, int32_t rows, int32_t dim, const float* x_dev, const float* residual_dev,
+                 const float* weight_dev, float eps, float* sum_dev, float* y_dev, uint8_t* y_fp8_dev,
+                 float* y_scale_dev) {
+    gsp::clear_error();
+    if (!ctx) return gsp::fail(GSP_E_INVALID_ARG, "ctx is NULL");
+    if (rows < 0 || dim < 1) return gsp::fail(GSP_E_INVALID_ARG, "rows must be >= 0 and dim >= 1 (got %d, %d)", rows, dim);
+    if (!(eps >= 0.0f) || !std::isfinite(eps)) return gsp::fail(GSP_E_INVALID_ARG, "eps must be finite and >= 0");
+    if (!y_fp8_dev != !y_scale_dev) return gsp::fail(GSP_E_INVALID_ARG, "codes and scales come together");
+    if (!sum_dev && !y_dev && !y_fp8_dev) return gsp::fail(GSP_E_INVALID_ARG, "no output is asked for");
+    if (sum_dev && !residual_dev) return gsp::fail(GSP_E_INVALID_ARG, "the sum needs a residual");
+    if (rows == 0) return GSP_OK;
+    if (!x_dev || !weight_dev) return gsp::fail(GSP_E_INVALID_ARG, "x/weight is NULL");
+    if (!is_aligned(x_dev, 4) || !is_aligned(residual_dev, 4) || !is_aligned(weight_dev, 4) || !is_aligned(sum_dev, 4) ||
+        !is_aligned(y_dev, 4) || !is_aligned(y_scale_dev, 4))
+        return gsp::fail(GSP_E_INVALID_ARG, "fp32 buffers must be 4-byte aligned");
+    const int64_t cells = (int64_t)rows * dim;
+    const Span in[] = {{x_dev, 4 * cells}, {residual_dev, 4 * cells}, {weight_dev, 4 * (int64_t)dim}};
+    const Span out[] = {{sum_dev, 4 * cells}, {y_dev, 4 * cells}, {y_fp8_dev, cells}, {y_scale_dev, 4 * (int64_t)rows}};
+    for (int i = 0; i < 4; ++i) {
+        for (int j = 0; j < 3; ++j) {
+            const bool in_place = i < 2 && j < 2 && out[i].p == in[j].p;
+            if (overlap(out[i], in[j]) && !in_place)
+                return gsp::fail(GSP_E_INVALID_ARG, "an output overlaps an input (sum and y may be x or the residual itself)");
+        }
+        for (int j = 0; j < i; ++j)
+            if (overlap(out[i], out[j])) return gsp::fail(GSP_E_INVALID_ARG, "two outputs overlap");
+    }
+    int rc = set_device(ctx);
+    if (rc) return rc;
+    gsp::RmsNormArgs a{};
+    a.x = x_dev;
+    a.residual = residual_dev;
+    a.weight = weight_dev;
+    a.sum = sum_dev;
+    a.y = y_dev;
+    a.codes = y_fp8_dev;
+    a.scale = y_scale_dev;
+    a.eps = eps;
+    a.rows = rows;
+    a.dim = dim;
+    return check_hip(gsp::launch_rms_norm(a, ctx->stream), "rms_norm launch");
+}
+
+int gsp_quantize_fp8(gsp_ctx* ctx, int32_t act, int32_t rows, int32_t dim, int64_t stride, const float* a_dev,
+                     const float* b_dev, uint8_t* y_fp8_dev, float* y_scale_dev) {
+    gsp::clear_error();
+    if (!ctx) return gsp::fail(GSP_E_INVALID_ARG, "ctx is NULL");
+    if (act != GSP_ACT_NONE && act != GSP_ACT_SILU_MUL) return gsp::fail(GSP_E_INVALID_ARG, "unknown activation %d", act);
+    if (rows < 0 || dim < 1) return gsp::fail(GSP_E_INVALID_ARG, "rows must be >= 0 and dim >= 1 (got %d, %d)", rows, dim);
+    if (stride < dim || stride > INT64_MAX / 8 / std::max(rows, 1))
+        return gsp::fail(GSP_E_INVALID_ARG, "row stride %lld does not fit %d rows of dim %d", (long long)stride, rows, dim);
+    if (rows == 0) return GSP_OK;
+    if (!a_dev || !y_fp8_dev || !y_scale_dev) return gsp::fail(GSP_E_INVALID_ARG, "NULL argument");
+    if ((act == GSP_ACT_NONE) != !b_dev) return gsp::fail(GSP_E_INVALID_ARG, "b goes with the gated activation only");
+    if (!is_aligned(a_dev, 4) || !is_aligned(b_dev, 4) || !is_aligned(y_scale_dev, 4))
+        return gsp::fail(GSP_E_INVALID_ARG, "fp32 buffers must be 4-byte aligned");
+    const int64_t bytes = ((int64_t)(rows - 1) * stride + dim) * 4;
+    const Span a_in{a_dev, bytes}, b_in{b_dev, bytes}, codes{y_fp8_dev, (int64_t)rows * dim}, scale{y_scale_dev, 4 * (int64_t)rows};
+    if (overlap(codes, a_in) || overlap(codes, b_in) || overlap(scale, a_in) || overlap(scale, b_in) || overlap(codes, scale))
+        return gsp::fail(GSP_E_INVALID_ARG, "the outputs overlap an input or each other");
+    int rc = set_device(ctx);
+    if (rc) return rc;
+    gsp::QuantizeArgs q{};
+    q.a = a_dev;
+    q.b = b_dev;
+    q.codes = y_fp8_dev;
+    q.scale = y_scale_dev;
+    q.stride = stride;
+    q.rows = rows;
+    q.dim = dim;
+    return check_hip(gsp::launch_quantize_fp8(q, ctx->stream), "quantize_fp8 launch");
+}
+
+int gsp_matmul_batch_fp8(gsp_ctx* ctx, int32_t w_type, const void* w_dev, const uint8_t* x_dev,
+                         const float* x_scale_dev, float* y_dev, int32_t in_dim, int32_t out_dim, int32_t batch) {
+    gsp::clear_error();
+    if (!ctx) return gsp::fail(GSP_E_INVALID_ARG, "ctx is NULL");
+    if (in_dim < 0 || out_dim < 0 || batch < 0)
+        return gsp::fail(GSP_E_INVALID_ARG, "negative size (inDim %d, outDim %d, batch %d)", in_dim, out_dim, batch);
+    if (batch == 0 || out_dim == 0) return GSP_OK;
+    if (!w_dev || !x_dev || !x_scale_dev || !y_dev) return gsp::fail(GSP_E_INVALID_ARG, "NULL argument");
+    if (w_type != GSP_WTYPE_Q4_0 && w_type != GSP_WTYPE_Q4_1 && w_type != GSP_WTYPE_Q4_K)
+        return gsp::fail(GSP_E_UNSUPPORTED, "weight type %d: only Q4_0 (%d), Q4_1 (%d) and Q4_K (%d) take 8-bit activations",
+                         w_type, GSP_WTYPE_Q4_0, GSP_WTYPE_Q4_1, GSP_WTYPE_Q4_K);
+    const int32_t unit = w_type == GSP_WTYPE_Q4_K ? 256 : 64;
+    if (in_dim == 0 || in_dim % unit != 0)
+        return gsp::fail(GSP_E_UNSUPPORTED, "inDim must be a positive multiple of %d for weight type %d (got %d)", unit,
+                         w_type, in_dim);
+    if (!is_aligned(w_dev, 4) || !is_aligned(x_dev, 16) || !is_aligned(x_scale_dev, 4) || !is_aligned(y_dev, 4))
+        return gsp::fail(GSP_E_INVALID_ARG, "weights must be 4-byte aligned, x 16-byte aligned, scales and y 4-byte aligned");
+    gsp::MatmulFp8Args a{};
+    a.w = w_dev;
+    a.x = x_dev;
+    a.x_scale = x_scale_dev;
+    a.y = y_dev;
+    a.row_bytes = gsp::matmul_fp8_row_bytes(w_type, in_dim);
+    a.in_dim = in_dim;
+    a.out_dim = out_dim;
+    a.batch = batch;
+    const Span y{y_dev, 4 * (int64_t)batch * out_dim};
+    if (overlap(y, Span{w_dev, a.row_bytes * out_dim}) || overlap(y, Span{x_dev, (int64_t)batch * in_dim}) ||
+        overlap(y, Span{x_scale_dev, 4 * (int64_t)batch}))
+        return gsp::fail(GSP_E_INVALID_ARG, "y overlaps another argument");
+    int rc = set_device(ctx);
+    if (rc) return rc;
+    return check_hip(gsp::launch_matmul_fp8(w_type, a, ctx->stream), "matmul_fp8 launch");
 }
 
 // Q8_0 and K-quant products with at least this many outputs (batch x out_dim)

@@ -52,6 +52,12 @@ SPLIT_RECORDS = 0
 SPLIT_IN_TILE = 1
 ROPE_PAIRS = 0
 ROPE_HALVES = 1
+MROPE_SECTIONS = 0
+MROPE_INTERLEAVED = 1
+MROPE_MAX_AXES = 4
+ACT_NONE = 0      # quantize_fp8: a
+ACT_SILU_MUL = 1  # a / (1 + exp(-a)) * b
+WTYPE_Q4_0, WTYPE_Q4_1 = 2, 3  # GGUF tensor type ids that gsp_matmul_batch_fp8 takes beside WTYPE_Q4_K
 WTYPE_F32, WTYPE_Q8_0, WTYPE_Q4_K, WTYPE_Q6_K = 0, 8, 12, 14  # GGUF tensor type ids (gsp_matmul_batch)
 BLOCK_SIZE = 16
 NOALLOC_SCRATCH_BYTES = 16 << 20  # GSP_NOALLOC_SCRATCH_BYTES: fixed scratch of attention_step_noalloc per GPU
@@ -172,6 +178,16 @@ class RopeSpec(ctypes.Structure):
     ]
 
 
+class MRopeSpec(ctypes.Structure):
+    """gsp_mrope_spec: the rotation, and which axis' position turns which pairs."""
+    _fields_ = [
+        ("rope", RopeSpec),
+        ("n_axes", i32),
+        ("sections", i32 * MROPE_MAX_AXES),
+        ("layout", i32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/glacier_paged.h.
 _SIGNATURES = {
     "gsp_last_error": (ctypes.c_char_p, []),
@@ -192,6 +208,13 @@ _SIGNATURES = {
     "gsp_pool_write_tokens": (ctypes.c_int, [vp, vp, i32, i32, i32p, i32p, vp, vp]),
     "gsp_rope_write_tokens": (ctypes.c_int, [vp, vp, i32, i32, i32p, i32p, i32p, i32, ctypes.c_float, i32, vp, vp, vp]),
     "gsp_matmul_batch": (ctypes.c_int, [vp, i32, vp, vp, vp, i32, i32, i32]),
+    "gsp_matmul_batch_fp8": (ctypes.c_int, [vp, i32, vp, vp, vp, vp, i32, i32, i32]),
+    "gsp_rms_norm": (ctypes.c_int, [vp, i32, i32, vp, vp, vp, ctypes.c_float, vp, vp, vp, vp]),
+    "gsp_quantize_fp8": (ctypes.c_int, [vp, i32, i32, i32, ctypes.c_int64, vp, vp, vp, vp]),
+    "gsp_mrope_write_step": (
+        ctypes.c_int,
+        [vp, vp, i32, i32, ctypes.POINTER(MRopeSpec), vp, vp, ctypes.c_int64, vp, vp, ctypes.c_int64, vp, ctypes.c_int64],
+    ),
     "gsp_pool_write_step": (ctypes.c_int, [vp, vp, i32, vp, vp]),
     "gsp_rope_write_step": (ctypes.c_int, [vp, vp, i32, i32, ctypes.c_float, i32, vp, vp, vp]),
     "gsp_rope_write_tokens_ex": (
@@ -322,6 +345,28 @@ class Context:
         y[b][o] = sum_i W[o][i] x[b][i], W as F32, Q8_0, Q4_K or Q6_K rows (WTYPE_*)."""
         _check(self._lib.gsp_matmul_batch(self._h, int(w_type), vp(w_ptr), vp(x_ptr), vp(y_ptr), int(in_dim),
                                           int(out_dim), int(batch)))
+
+    def matmul_batch_fp8(self, w_type: int, w_ptr: int, x_ptr: int, x_scale_ptr: int, y_ptr: int, in_dim: int,
+                         out_dim: int, batch: int) -> None:
+        """matmul_batch on e4m3 activations with one scale a row (gsp_matmul_batch_fp8):
+        y[b][o] = x_scale[b] sum_i W[o][i] x[b][i], W as Q4_0, Q4_1 or Q4_K rows (WTYPE_*)."""
+        _check(self._lib.gsp_matmul_batch_fp8(self._h, int(w_type), w_ptr, x_ptr, x_scale_ptr, y_ptr, int(in_dim),
+                                              int(out_dim), int(batch)))
+
+    def rms_norm(self, rows: int, dim: int, x_ptr: int, weight_ptr: int, eps: float, residual_ptr: int = 0,
+                 sum_ptr: int = 0, y_ptr: int = 0, y_fp8_ptr: int = 0, y_scale_ptr: int = 0) -> None:
+        """RMS norm of x (+ residual) with the results whose pointers are given (gsp_rms_norm): the sum, y in
+        fp32, y's e4m3 codes and row scales."""
+        _check(self._lib.gsp_rms_norm(self._h, int(rows), int(dim), x_ptr, residual_ptr or None, weight_ptr,
+                                      float(eps), sum_ptr or None, y_ptr or None, y_fp8_ptr or None,
+                                      y_scale_ptr or None))
+
+    def quantize_fp8(self, act: int, rows: int, dim: int, stride: int, a_ptr: int, b_ptr: int, y_fp8_ptr: int,
+                     y_scale_ptr: int) -> None:
+        """Rows of a (ACT_NONE, b_ptr 0) or silu(a) * b (ACT_SILU_MUL) into e4m3 codes and row scales
+        (gsp_quantize_fp8); rows of a and b start `stride` floats apart."""
+        _check(self._lib.gsp_quantize_fp8(self._h, int(act), int(rows), int(dim), int(stride), a_ptr, b_ptr or None,
+                                          y_fp8_ptr, y_scale_ptr))
 
     def set_split_pages(self, pages: int) -> None:
         """Largest split-KV unit in pages for the next pack (0: sized from the step and device)."""
@@ -558,6 +603,17 @@ class Pool:
         _check(load().gsp_rope_write_step(self._ctx.handle, self._h, int(layer), int(n_heads), float(freq_base),
                                           int(style), vp(q_ptr), vp(k_ptr), vp(v_ptr)))
 
+    def mrope_write_step(self, layer: int, n_heads: int, rope: "MRope", positions_ptr: int, q_ptr: int,
+                         q_out_ptr: int, k_ptr: int, v_ptr: int, q_stride: int = 0, k_stride: int = 0,
+                         v_stride: int = 0) -> None:
+        """rope_write_step_ex with a position per axis for every query token (gsp_mrope_write_step):
+        positions [n_axes][total_q] int32 on the device; rows of q, k and v start the given number of
+        floats apart (0: dense), the turned q goes to q_out, dense."""
+        spec = rope.spec(self.desc.head_dim)
+        _check(load().gsp_mrope_write_step(self._ctx.handle, self._h, int(layer), int(n_heads), ctypes.byref(spec),
+                                           positions_ptr, q_ptr or None, int(q_stride), q_out_ptr or None, k_ptr,
+                                           int(k_stride), v_ptr, int(v_stride)))
+
     def copy_block_data(self, src: int, dst: int, valid_tokens: int) -> None:
         """PagedBlockPool.CopyBlockData (PagedBlockPool.cs:304-327) on the device."""
         _check(load().gsp_pool_copy_block(self._ctx.handle, self._h, int(src), int(dst), int(valid_tokens)))
@@ -588,6 +644,23 @@ class Rope:
         tab = lambda t: fp32() if t is None else t.ctypes.data_as(fp32)
         return RopeSpec(self.freq_base, self.style, self.rope_dim, self.mscale, tab(self.inv_freq),
                         tab(self.freq_factors))
+
+
+class MRope(Rope):
+    """A rotation by positions of several axes: `sections` pairs of a head turn with each axis, in
+    turn (MROPE_SECTIONS) or dealt out one by one (MROPE_INTERLEAVED); the rest is Rope's."""
+
+    def __init__(self, freq_base: float, sections: Sequence[int], style: int = 0, layout: int = 0, rope_dim: int = 0,
+                 inv_freq=None, freq_factors=None, mscale: float = 0.0):
+        super().__init__(freq_base, style, rope_dim, inv_freq, freq_factors, mscale)
+        self.sections = [int(n) for n in sections]
+        self.layout = int(layout)
+        if len(self.sections) > MROPE_MAX_AXES:
+            raise ValueError(f"{len(self.sections)} axes; at most {MROPE_MAX_AXES}")
+
+    def spec(self, head_dim: int) -> MRopeSpec:
+        return MRopeSpec(super().spec(head_dim), len(self.sections), (i32 * MROPE_MAX_AXES)(*self.sections),
+                         self.layout)
 
 
 def prefix_hash(parent_hash: int, tokens) -> int:

@@ -229,6 +229,98 @@ int gsp_rope_write_step_ex(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, int32_t 
                            const gsp_rope_spec* rope, float* q_dev, const float* k_dev,
                            const float* v_dev);
 
+/* Rotary positions of several axes (an image token's time, row and column)
+ * and the packed step's K/V write, in one call: gsp_rope_write_step_ex where
+ * each pair of a head turns with one of n_axes positions of its token, which
+ * the caller gives, while the slot stays that of the token's place in its row.
+ *   rope      the rotation: freq_base, style, rope_dim, mscale and the tables,
+ *             as above.  Pair j turns by positions[axis(j)][i] times its rate.
+ *   n_axes    1 to GSP_MROPE_MAX_AXES.
+ *   sections  pairs of each axis; they add up to rope_dim / 2 (of the others
+ *             none is read).
+ *   layout    GSP_MROPE_SECTIONS: the first sections[0] pairs turn with axis 0,
+ *             the next sections[1] with axis 1, and so on.
+ *             GSP_MROPE_INTERLEAVED: pair j turns with axis j % n_axes while
+ *             that axis has pairs left (j < n_axes * sections[j % n_axes]), and
+ *             with axis 0 otherwise; axis a > 0 must find its pairs within the
+ *             head (n_axes * (sections[a] - 1) + a < rope_dim / 2).
+ * positions_dev is [n_axes][total_q] int32 on the device, any values.  q_dev,
+ * k_dev and v_dev are rows of q_stride, k_stride and v_stride floats, one for
+ * each query token of the step (0: dense rows), so that the columns of one
+ * fused projection can be given as they lie.  The turned Q goes to q_out_dev,
+ * dense [total_q][n_heads][head_dim], which may be q_dev itself if that is
+ * dense, and may not overlap any input otherwise (GSP_E_INVALID_ARG).  n_heads
+ * 0 leaves Q out.  K and V go where gsp_rope_write_step stores them.  Tables and
+ * graph capture are as for gsp_rope_write_step_ex. */
+#define GSP_MROPE_SECTIONS 0
+#define GSP_MROPE_INTERLEAVED 1
+#define GSP_MROPE_MAX_AXES 4
+typedef struct gsp_mrope_spec {
+  gsp_rope_spec rope;
+  int32_t n_axes;
+  int32_t sections[GSP_MROPE_MAX_AXES];
+  int32_t layout;
+} gsp_mrope_spec;
+
+int gsp_mrope_write_step(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, int32_t n_heads, const gsp_mrope_spec* spec,
+                         const int32_t* positions_dev, const float* q_dev, int64_t q_stride, float* q_out_dev,
+                         const float* k_dev, int64_t k_stride, const float* v_dev, int64_t v_stride);
+
+/* ------------------------------------------------------------------------ */
+/* 8-bit activations: norm, quantiser and projections around the attention   */
+/* (the reference's RMSNorm, FFN gate and MatMulBatch calls,                 */
+/* PagedTransformerRunner.cs:588-603,659).  Codes are OCP e4m3 bytes, one    */
+/* fp32 scale a row: value = scale * code.  All pointers are device          */
+/* pointers; the calls only enqueue one kernel on the context's stream, keep */
+/* no workspace and can be captured.                                         */
+/* ------------------------------------------------------------------------ */
+
+/* The root-mean-square norm of `rows` rows of `dim` fp32 values, with the
+ * residual's addition before it:
+ *   s = x + residual (residual NULL: x),  y = s * weight / sqrt(mean(s^2) + eps).
+ * Results, each left out with NULL (one at least is asked for): sum_dev, s in
+ * fp32, which needs a residual; y_dev, y in fp32; y_fp8_dev with y_scale_dev,
+ * y's codes and each row's scale max(max |y|, 2^-100) / 448, every code the
+ * e4m3 value nearest to y / scale.  A row that holds a NaN gets NaN codes or a
+ * NaN scale; one that holds an infinity gets a NaN or zero for every value, as
+ * the formula does.  sum_dev and y_dev may each be x_dev or residual_dev
+ * itself; every other overlap of an output with another argument is refused
+ * (GSP_E_INVALID_ARG).  eps is finite and >= 0.  rows may be 0; dim is at least
+ * 1.  Rows of any length and 4-byte alignment are taken; 16-byte aligned
+ * buffers with dim a multiple of 4 are read and written 16 bytes at a time. */
+int gsp_rms_norm(gsp_ctx* ctx, int32_t rows, int32_t dim, const float* x_dev, const float* residual_dev,
+                 const float* weight_dev, float eps, float* sum_dev, float* y_dev, uint8_t* y_fp8_dev,
+                 float* y_scale_dev);
+
+/* Rows of fp32 activations into codes and scales (as y's of gsp_rms_norm).
+ * GSP_ACT_NONE quantises a_dev (b_dev NULL), GSP_ACT_SILU_MUL
+ * a / (1 + exp(-a)) * b.  Row i starts at a_dev + i * stride (and b_dev + i *
+ * stride), stride >= dim in floats, so that the halves of one fused gate and up
+ * projection are given as they lie; the codes are dense, [rows][dim].  The
+ * outputs must not overlap the inputs or each other. */
+#define GSP_ACT_NONE 0
+#define GSP_ACT_SILU_MUL 1
+int gsp_quantize_fp8(gsp_ctx* ctx, int32_t act, int32_t rows, int32_t dim, int64_t stride, const float* a_dev,
+                     const float* b_dev, uint8_t* y_fp8_dev, float* y_scale_dev);
+
+/* gsp_matmul_batch on 8-bit activations: y[b][o] = x_scale[b] * sum_i W[o][i] *
+ * x[b][i] for b < batch, o < out_dim, x_dev being [batch][in_dim] codes (16-byte
+ * aligned), x_scale_dev [batch] and y_dev [batch][out_dim] fp32, overwritten; y
+ * must not overlap another argument.  Weight types, rows in their GGUF bytes
+ * (4-byte aligned): Q4_K as above, and the blocks of 32 weights Q4_0
+ * (GSP_WTYPE_Q4_0, 18 bytes: fp16 d, then 16 bytes whose low halves are weights
+ * 0 to 15 and whose high halves are 16 to 31, w = d * (q - 8)) and Q4_1
+ * (GSP_WTYPE_Q4_1, 20 bytes: fp16 d, fp16 m, the same 16 bytes, w = d * q + m).
+ * The product of weights and codes is exact, sums are fp32: no rounding of x or
+ * W is added to the codes' own.  in_dim is a multiple of 64 (256 for Q4_K;
+ * GSP_E_UNSUPPORTED otherwise, as for other weight types).  Results are the
+ * same bit for bit on every call, and a row's do not depend on the other rows
+ * of its batch in value, only in the order of their sums. */
+#define GSP_WTYPE_Q4_0 2
+#define GSP_WTYPE_Q4_1 3
+int gsp_matmul_batch_fp8(gsp_ctx* ctx, int32_t w_type, const void* w_dev, const uint8_t* x_dev,
+                         const float* x_scale_dev, float* y_dev, int32_t in_dim, int32_t out_dim, int32_t batch);
+
 /* Weight types of gsp_matmul_batch: the GGUF tensor type ids. */
 #define GSP_WTYPE_F32 0
 #define GSP_WTYPE_Q8_0 8
