@@ -227,13 +227,22 @@ struct MatmulFp8Args {
     const uint8_t* x;      // [batch][in_dim] e4m3
     const float* x_scale;  // [batch]
     float* y;              // [batch][out_dim]
+    float* partials;       // [splits][batch][out_dim] with several splits of K, else null
     int64_t row_bytes;
+    int32_t units_per_split;  // 256 of K each; launch_matmul_fp8 sets it
     int32_t in_dim;        // a multiple of 64 (Q4_K: of 256)
     int32_t out_dim;
     int32_t batch;
 };
+// The kernel that a product takes, and the ranges of K that share an output (several only with a tile form).
+struct MatmulFp8Plan {
+    enum { kStream = 0, kTile128, kTile64, kTile32 };
+    int32_t form = kStream;
+    int32_t splits = 1;
+};
+MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, int cus);
 int64_t matmul_fp8_row_bytes(int32_t w_type, int32_t in_dim);
-hipError_t launch_matmul_fp8(int32_t w_type, const MatmulFp8Args& a, hipStream_t stream);
+hipError_t launch_matmul_fp8(int32_t w_type, const MatmulFp8Args& a, const MatmulFp8Plan& plan, hipStream_t stream);
 
 // Projection GEMM (gsp_matmul.hip): y[b][o] = sum_i W[o][i] x[b][i].
 constexpr int kWeightF32 = 0;   // GGUF type ids

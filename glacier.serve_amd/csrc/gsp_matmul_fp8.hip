@@ -23,6 +23,7 @@
 // operands agree, so lanes load long contiguous pieces (64 weights of a row,
 // 16 activations) and a 4 x 4 transposition among the four lanes of a column
 // (four register swaps, no LDS) deals every lane its dword of each piece.
+#include <cmath>
 #include <type_traits>
 
 #include "gsp_internal.h"
@@ -34,7 +35,6 @@ namespace {
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-typedef u4 u4_al4 __attribute__((aligned(4)));
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -87,7 +87,7 @@ __device__ inline Terms x_terms(uint32_t lo, uint32_t hi) {
     const auto two = [](uint32_t w, auto high) {
         return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, decltype(high)::value));
     };
-    return Terms{{two(lo, std::false_type{}), two(hi, std::false_type{}), two(lo, std::true_type{}),
+    return Terms{{two(lo, std::false_type{}), two(lo, std::true_type{}), two(hi, std::false_type{}),
                   two(hi, std::true_type{})}};
 }
 
@@ -96,58 +96,33 @@ __device__ inline Terms splat_terms(uint32_t half) {
     const uint32_t w = half * 0x10001u;
     return Terms{{w, w, w, w}};
 }
-constexpr uint32_t kOne = 0x3c00, kMinus8 = 0x8080;  // 1, -8 / kCode
+constexpr uint32_t kOne = 0x0010, kMinus8 = 0x8080;  // 1 / kCode, -8 / kCode
 
 // Bytes 0 2 1 3 of a dword: the two 16-bit lanes of a mask then hold neighbours.
 __device__ inline uint32_t deal_bytes(uint32_t w) { return __builtin_amdgcn_perm(w, w, 0x03010200u); }
 
-// A unit is 256 weights of each of 16 rows: lane (n, j) holds the j-th 64 of
-// row n as they lie in memory.
+// A unit is 256 weights of each of 16 rows, as they lie in memory: 128 or 160
+// bytes a row and its scales.  Lane (n, j) reads the j-th 64 of row n from LDS.
 template <int WT>
-struct Unit;
+struct Unit {
+    static constexpr bool kMins = WT != GSP_WTYPE_Q4_0;
+    static constexpr int kRow = WT == GSP_WTYPE_Q4_1 ? 160 : 144;
+    // Q4_0, Q4_1: a pair of blocks.  Q4_K: d | dmin, 12 bytes of scales and mins, 32 bytes of quants.
+    static constexpr int kWords = WT == GSP_WTYPE_Q4_0 ? 9 : WT == GSP_WTYPE_Q4_1 ? 10 : 12;
+    uint32_t w[kWords];
 
-template <>
-struct Unit<GSP_WTYPE_Q4_0> {
-    static constexpr int kPairBytes = 36;
-    static constexpr bool kMins = false;
-    uint32_t w[9];
-    __device__ inline void load(const uint8_t* row, int64_t pair) {
-        const uint8_t* p = row + pair * kPairBytes;
-        const u4 a = *reinterpret_cast<const u4_al4*>(p);
-        const u4 b = *reinterpret_cast<const u4_al4*>(p + 16);
-        w[8] = *reinterpret_cast<const uint32_t*>(p + 32);
+    __device__ inline void read(const uint8_t* rows, int n, int j) {
+        const uint8_t* p = rows + n * kRow;
+        if constexpr (WT == GSP_WTYPE_Q4_K) {
+            const u4 h = *reinterpret_cast<const u4*>(p);
+            const u4 a = *reinterpret_cast<const u4*>(p + 16 + 32 * j);
+            const u4 b = *reinterpret_cast<const u4*>(p + 32 + 32 * j);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = a[i], w[4 + i] = b[i];
-    }
-};
-
-template <>
-struct Unit<GSP_WTYPE_Q4_1> {
-    static constexpr int kPairBytes = 40;
-    static constexpr bool kMins = true;
-    uint32_t w[10];
-    __device__ inline void load(const uint8_t* row, int64_t pair) {
-        const uint8_t* p = row + pair * kPairBytes;
-        const u4 a = *reinterpret_cast<const u4_al4*>(p);
-        const u4 b = *reinterpret_cast<const u4_al4*>(p + 16);
-        w[8] = *reinterpret_cast<const uint32_t*>(p + 32);
-        w[9] = *reinterpret_cast<const uint32_t*>(p + 36);
+            for (int i = 0; i < 4; ++i) w[i] = h[i], w[4 + i] = a[i], w[8 + i] = b[i];
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = a[i], w[4 + i] = b[i];
-    }
-};
-
-template <>
-struct Unit<GSP_WTYPE_Q4_K> {
-    static constexpr bool kMins = true;
-    uint32_t w[12];  // d | dmin, 12 bytes of scales and mins, the quarter's 32 bytes of quants
-    __device__ inline void load(const uint8_t* row, int64_t pair) {
-        const uint8_t* p = row + (pair >> 2) * 144;
-        const u4 h = *reinterpret_cast<const u4_al4*>(p);
-        const u4 a = *reinterpret_cast<const u4_al4*>(p + 16 + 32 * (pair & 3));
-        const u4 b = *reinterpret_cast<const u4_al4*>(p + 32 + 32 * (pair & 3));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = h[i], w[4 + i] = a[i], w[8 + i] = b[i];
+            for (int i = 0; i < kWords; ++i) w[i] = *reinterpret_cast<const uint32_t*>(p + 4 * kWords * j + 4 * i);
+        }
     }
 };
 
@@ -158,7 +133,7 @@ template <int WT>
 struct Dealt {
     uint32_t q[2][4];
     uint32_t s[2][4];
-    float d, dmin;  // Q4_K: of the super-block, d times kCode
+    float d, dmin;  // Q4_K: of the super-block
 
     __device__ inline void deal(const Unit<WT>& u) {
         if constexpr (WT == GSP_WTYPE_Q4_0) {
@@ -177,7 +152,7 @@ struct Dealt {
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) q[0][i] = deal_bytes(u.w[4 + i]), q[1][i] = deal_bytes(u.w[8 + i]);
-            d = half_lo(u.w[0]) * kCode;
+            d = half_lo(u.w[0]);
             dmin = half_hi(u.w[0]);
             // Groups 2j and 2j + 1: two 6-bit scales and two 6-bit mins into one dword.
             const int j = (threadIdx.x >> 4) & 3;
@@ -190,20 +165,54 @@ struct Dealt {
         transpose4(q[0][0], q[0][1], q[0][2], q[0][3]);
         transpose4(q[1][0], q[1][1], q[1][2], q[1][3]);
     }
+    // Quants times 1 / kCode.
     __device__ inline Terms terms(int t, int h) const {
         if constexpr (WT == GSP_WTYPE_Q4_K) {
-            // 4j .. 4j + 3 from q[0], 16 + 4j .. from q[1].
             const uint32_t a = q[0][t], b = q[1][t];
-            if (h) return Terms{{a & kNib, b & kNib, (a >> 8) & kNib, (b >> 8) & kNib}};
-            return Terms{{(a << 4) & kNib, (b << 4) & kNib, (a >> 4) & kNib, (b >> 4) & kNib}};
+            if (h) return Terms{{a & kNib, (a >> 8) & kNib, b & kNib, (b >> 8) & kNib}};
+            return Terms{{(a << 4) & kNib, (a >> 4) & kNib, (b << 4) & kNib, (b >> 4) & kNib}};
         }
         const uint32_t a = q[h][t];
-        return Terms{{(a << 4) & kNib, a & kNib, (a >> 4) & kNib, (a >> 8) & kNib}};
+        return Terms{{(a << 4) & kNib, (a >> 4) & kNib, a & kNib, (a >> 8) & kNib}};
     }
-    // The group's scale, times kCode, and what the sum of x enters with.
+    // What the tile form multiplies activations by, as normal fp16 numbers formed from 1024 + 16 q in one fused
+    // step: q - 8 (Q4_0), q (Q4_1), or q times the group's 6-bit scale, an exact integer up to 945 (Q4_K).  mask:
+    // kNib in a register, for one instruction with the or.
+    __device__ inline Terms operand(int t, int h, uint32_t mask) const {
+        h2 f = {0.0625f16, 0.0625f16}, c = {-64.f16, -64.f16};
+        if constexpr (WT == GSP_WTYPE_Q4_0) c = h2{-72.f16, -72.f16};
+        if constexpr (WT == GSP_WTYPE_Q4_K) {
+            const float sc = (float)((s[0][t] >> (8 * h)) & 0xffu) * 0.0625f;
+            f = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(sc, sc));
+            c = f * h2{-1024.f16, -1024.f16};
+        }
+        const auto make = [&](uint32_t w) {
+            return __builtin_bit_cast(
+                uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & mask) | 0x64006400u), f, c));
+        };
+        const uint32_t a = WT == GSP_WTYPE_Q4_K ? q[0][t] : q[h][t], b = WT == GSP_WTYPE_Q4_K ? q[1][t] : a;
+        if (WT == GSP_WTYPE_Q4_K && h) return Terms{{make(a), make(a >> 8), make(b), make(b >> 8)}};
+        if (WT == GSP_WTYPE_Q4_K) return Terms{{make(a << 4), make(a >> 4), make(b << 4), make(b >> 4)}};
+        return Terms{{make(a << 4), make(a >> 4), make(a), make(a >> 8)}};
+    }
+    // The unit's eight minimums as fp16, m (Q4_1) or the 6-bit integer (Q4_K), for the lanes where keep is all ones.
+    __device__ inline Terms minimums(uint32_t keep) const {
+        Terms t;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (WT == GSP_WTYPE_Q4_K) {
+                const float lo = (float)((s[0][i] >> 16) & 0xffu), hi = (float)(s[0][i] >> 24);
+                t.r[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi)) & keep;
+            } else {
+                t.r[i] = __builtin_amdgcn_perm(s[1][i], s[0][i], 0x07060302u) & keep;
+            }
+        }
+        return t;
+    }
+    // The group's scale, and what the sum of x enters with.
     __device__ inline float scale(int t, int h) const {
-        if constexpr (WT == GSP_WTYPE_Q4_0) return (h ? half_hi(s[0][t]) : half_lo(s[0][t])) * kCode;
-        if constexpr (WT == GSP_WTYPE_Q4_1) return half_lo(s[h][t]) * kCode;
+        if constexpr (WT == GSP_WTYPE_Q4_0) return h ? half_hi(s[0][t]) : half_lo(s[0][t]);
+        if constexpr (WT == GSP_WTYPE_Q4_1) return half_lo(s[h][t]);
         return d * (float)((s[0][t] >> (8 * h)) & 0xffu);
     }
     __device__ inline float least(int t, int h) const {
@@ -213,24 +222,71 @@ struct Dealt {
     }
 };
 
+// BYTES of every lane into LDS, one lane's behind the other's from `to` on.
+template <int BYTES>
+__device__ inline void load_to_lds(const uint8_t* from, uint8_t* to) {
+    const auto f = (const __attribute__((address_space(1))) void*)from;
+    const auto t = (__attribute__((address_space(3))) void*)to;
+    if constexpr (BYTES == 16)
+        __builtin_amdgcn_global_load_lds(f, t, 16, 0, 0);
+    else
+        __builtin_amdgcn_global_load_lds(f, t, 4, 0, 0);
+}
+
 // One workgroup: 16 * NT weight rows by 16 * MT batch rows.  Its waves share
 // the units of K, each with sums of its own, which are added in the order of
 // the waves at the end.
-template <int WT, int MT, int NT>
-__global__ __launch_bounds__(1024) void matmul_fp8_kernel(MatmulFp8Args a) {
-    extern __shared__ float part[];  // [waves][NT][MT][256]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+//
+// Each wave has a slot of LDS for one unit of weights and of activations.  Loads
+// go straight there, with neighbouring lanes on neighbouring bytes: a lane that
+// loaded what it multiplies would put each 16 bytes of an instruction on another
+// row, one cache access a lane.  The wave takes the landed unit into registers
+// and sends the next one's loads off before it computes.  AL: rows of weights are
+// 16-byte aligned and whole units; otherwise they are loaded 4 bytes a lane.
+template <int WT, int MT, int NT, int W, bool AL>
+__global__ __launch_bounds__(64 * W) void matmul_fp8_kernel(MatmulFp8Args a) {
+    constexpr int kRow = Unit<WT>::kRow, kTile = 16 * kRow, kSlot = NT * kTile + MT * 4096;
+    static_assert(W * kSlot >= W * NT * MT * 1024, "the partial sums take the slots' place");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[W * kSlot];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int n = lane & 15, j = lane >> 4;
     const int tiles_b = (a.batch + 16 * MT - 1) / (16 * MT);
     const int row0 = blockIdx.x / tiles_b * (16 * NT), b0 = blockIdx.x % tiles_b * (16 * MT);
     const int pairs = a.in_dim >> 6, units = (pairs + 3) >> 2;
-    const uint8_t* wrow[NT];
+    uint8_t* slot = lds + wave * kSlot;
+
+    // Where a lane's bytes of a tile lie: the tile's LDS image is 16 rows of kRow bytes, filled in the lanes' order.
+    const uint8_t* w0 = static_cast<const uint8_t*>(a.w);
+    const auto weight_at = [&](int i, int byte, int u) {
+        const int r = byte / kRow, c = byte % kRow;
+        const int64_t row = (int64_t)min(row0 + 16 * i + r, a.out_dim - 1) * a.row_bytes;
+        int64_t col = (int64_t)u * kRow + c;
+        if constexpr (!AL) col = min(col, a.row_bytes - 4);
+        return w0 + row + col;
+    };
+    // Piece p (16 bytes) of row r of activations goes to place p ^ r of the row, so that the reads below spread over
+    // the banks.  Bytes past the row's end are its last piece again and meet no product.
+    const auto x_at = [&](int m, int i, int u) {
+        const int r = 4 * i + (lane >> 4), p = (lane & 15) ^ r;
+        const int64_t row = (int64_t)min(b0 + 16 * m + r, a.batch - 1) * a.in_dim;
+        return a.x + row + min(u * 256 + p * 16, a.in_dim - 16);
+    };
+    const auto send = [&](int u) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-        wrow[i] = static_cast<const uint8_t*>(a.w) + (int64_t)min(row0 + 16 * i + n, a.out_dim - 1) * a.row_bytes;
-    const uint8_t* xrow[MT];
+        for (int i = 0; i < NT; ++i) {
+            uint8_t* to = slot + i * kTile;
+            constexpr int kWide = AL ? kTile / 1024 * 1024 : 0;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) xrow[m] = a.x + (int64_t)min(b0 + 16 * m + n, a.batch - 1) * a.in_dim + 16 * j;
+            for (int at = 0; at < kWide; at += 1024) load_to_lds<16>(weight_at(i, at + 16 * lane, u), to + at);
+#pragma unroll
+            for (int at = kWide; at < kTile; at += 256) load_to_lds<4>(weight_at(i, at + 4 * lane, u), to + at);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load_to_lds<16>(x_at(m, i, u), slot + NT * kTile + m * 4096 + i * 1024);
+        }
+    };
 
     f4 acc[NT][MT];
 #pragma unroll
@@ -238,57 +294,62 @@ __global__ __launch_bounds__(1024) void matmul_fp8_kernel(MatmulFp8Args a) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[i][m] = f4{0.f, 0.f, 0.f, 0.f};
     }
-    Unit<WT> next[NT];
-    if (wave < units) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i) next[i].load(wrow[i], min(4 * wave + j, pairs - 1));
-    }
+    if (wave < units) send(wave);
     for (int u = wave; u < units; u += waves) {
-        Dealt<WT> w[NT];
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the unit has landed
+        Unit<WT> raw[NT];
+        u4 xq[4][MT];
 #pragma unroll
-        for (int i = 0; i < NT; ++i) w[i].deal(next[i]);
-        if (u + waves < units) {
-#pragma unroll
-            for (int i = 0; i < NT; ++i) next[i].load(wrow[i], min(4 * (u + waves) + j, pairs - 1));
-        }
+        for (int i = 0; i < NT; ++i) raw[i].read(slot + i * kTile, n, j);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            if (4 * u + t < pairs) {
-                uint32_t x[MT][4];
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+                xq[t][m] = *reinterpret_cast<const u4*>(slot + NT * kTile + m * 4096 + n * 256 + ((4 * t + j) ^ n) * 16);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and is in registers: the slot may be overwritten
+        if (u + waves < units) send(u + waves);
+        Dealt<WT> w[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) w[i].deal(raw[i]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            if (!AL && 4 * u + t >= pairs) continue;
+            uint32_t x[MT][4];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[m][i] = xq[t][m][i];
+                transpose4(x[m][0], x[m][1], x[m][2], x[m][3]);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                Terms xt[MT];
+                f4 sx[MT];
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    const u4 v = *reinterpret_cast<const u4*>(xrow[m] + (int64_t)(4 * u + t) * 64);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[m][i] = v[i];
-                    transpose4(x[m][0], x[m][1], x[m][2], x[m][3]);
+                    xt[m] = x_terms(x[m][2 * h], x[m][2 * h + 1]);
+                    sx[m] = mfma(xt[m], splat_terms(Unit<WT>::kMins ? kOne : kMinus8), f4{0.f, 0.f, 0.f, 0.f});
                 }
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    Terms xt[MT];
-                    f4 sx[MT];
+                for (int i = 0; i < NT; ++i) {
+                    const Terms q = w[i].terms(t, h);
+                    const float sc = w[i].scale(t, h), mn = w[i].least(t, h);
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
-                        xt[m] = x_terms(x[m][2 * h], x[m][2 * h + 1]);
-                        sx[m] = mfma(xt[m], splat_terms(Unit<WT>::kMins ? kOne : kMinus8), f4{0.f, 0.f, 0.f, 0.f});
-                    }
+                        const f4 s = mfma(xt[m], q, Unit<WT>::kMins ? f4{0.f, 0.f, 0.f, 0.f} : sx[m]);
 #pragma unroll
-                    for (int i = 0; i < NT; ++i) {
-                        const Terms q = w[i].terms(t, h);
-                        const float sc = w[i].scale(t, h), mn = w[i].least(t, h);
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            const f4 s = mfma(xt[m], q, Unit<WT>::kMins ? f4{0.f, 0.f, 0.f, 0.f} : sx[m]);
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                acc[i][m][r] = fmaf(sc, s[r], acc[i][m][r]);
-                                if constexpr (Unit<WT>::kMins) acc[i][m][r] = fmaf(mn, sx[m][r], acc[i][m][r]);
-                            }
+                        for (int r = 0; r < 4; ++r) {
+                            acc[i][m][r] = fmaf(sc, s[r], acc[i][m][r]);
+                            if constexpr (Unit<WT>::kMins) acc[i][m][r] = fmaf(mn, sx[m][r], acc[i][m][r]);
                         }
                     }
                 }
             }
         }
     }
+    __syncthreads();  // every wave is done with its slot
+    float* part = reinterpret_cast<float*>(lds);  // [waves][NT][MT][256]
     // Lane (n, j) holds batch rows 4j .. 4j + 3 of weight row n.
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -305,24 +366,23 @@ __global__ __launch_bounds__(1024) void matmul_fp8_kernel(MatmulFp8Args a) {
         for (int v = 0; v < waves; ++v) s += part[v * (NT * MT * 256) + e];
         const int i = e / (MT * 256), m = e / 256 % MT;
         const int b = b0 + 16 * m + (e >> 4) % 16, o = row0 + 16 * i + (e & 15);
-        if (b < a.batch && o < a.out_dim) a.y[(int64_t)b * a.out_dim + o] = s * a.x_scale[b];
+        if (b < a.batch && o < a.out_dim) a.y[(int64_t)b * a.out_dim + o] = s * kCode * a.x_scale[b];
     }
 }
 
-template <int WT, int MT, int NT>
-hipError_t launch_form(MatmulFp8Args a, hipStream_t stream) {
-    const int units = (a.in_dim + 255) / 256;
-    const int most = std::min(16, 65536 / (NT * MT * 1024));
-    const int per = (units + most - 1) / most;
-    const int waves = (units + per - 1) / per;
+template <int WT, int MT, int NT, int W>
+hipError_t launch_form(MatmulFp8Args a, int waves, hipStream_t stream) {
+    const bool aligned = a.in_dim % 256 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
     // A launch holds fewer than 2^32 threads: very large batches take several.
     const int64_t tiles = ((int64_t)a.out_dim + 16 * NT - 1) / (16 * NT);
     const int64_t most_rows = std::max<int64_t>(1, (1 << 21) / tiles) * (16 * MT);
     for (int64_t left = a.batch; left > 0; left -= most_rows) {
         a.batch = (int32_t)std::min(left, most_rows);
         const uint32_t grid = (uint32_t)(tiles * ((a.batch + 16 * MT - 1) / (16 * MT)));
-        hipLaunchKernelGGL((matmul_fp8_kernel<WT, MT, NT>), dim3(grid), dim3(64 * waves), waves * NT * MT * 1024, stream,
-                           a);
+        if (aligned)
+            hipLaunchKernelGGL((matmul_fp8_kernel<WT, MT, NT, W, true>), dim3(grid), dim3(64 * waves), 0, stream, a);
+        else
+            hipLaunchKernelGGL((matmul_fp8_kernel<WT, MT, NT, W, false>), dim3(grid), dim3(64 * waves), 0, stream, a);
         a.x += (int64_t)a.batch * a.in_dim;
         a.x_scale += a.batch;
         a.y += (int64_t)a.batch * a.out_dim;
@@ -330,23 +390,366 @@ hipError_t launch_form(MatmulFp8Args a, hipStream_t stream) {
     return hipGetLastError();
 }
 
+// Keeps a value's computation from being moved behind this point, or folded into its uses.
+__device__ inline void pin(f4& v) { asm volatile("" : "+v"(v)); }
+__device__ inline void pin(float& v) { asm volatile("" : "+v"(v)); }
+
+// LDS traffic of the wave is done; the other waves' too after the barrier.
+// Loads to LDS stay in flight, which __syncthreads() would wait for.
+__device__ inline void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// The tile form, for batches that use an expanded weight many times: 16 * MT
+// batch rows by 16 * NT * WN weight rows a workgroup.  Activations are converted
+// once a workgroup into LDS, in the order the instruction's operands take, 128 of K
+// at a time in two buffers; each wave has its own weight rows, in a slot as above.
+//
+// The matrix and the vector units work beside each other: while the products of one
+// set (16 weight rows, all batch rows, one group) run, the previous set's sums are
+// scaled into the outputs' (Q4_0 and Q4_1: one fused multiply-add an output and group
+// is the vector unit's main work) and the next set's weights are expanded.  Q4_1's
+// minimum is a second product straight into the outputs' sums; Q4_K's scales are
+// integers within the operand, so that its sums and those of its minimums run over
+// the eight groups of a super-block in the matrix unit alone.
+template <int WT, int MT, int NT, int WN, int G, bool AL>
+__global__ __launch_bounds__(64 * WN) void matmul_fp8_tile_kernel(MatmulFp8Args a) {
+    constexpr int kRow = Unit<WT>::kRow, kTile = 16 * kRow;
+    constexpr int kSteps = 8 / G;                            // of a unit, G groups of 32 each
+    constexpr int kStep = MT * G * 1024;                     // LDS bytes of a step's activations
+    constexpr int kRowPieces = 2 * G;                        // 16-byte pieces of a row in a step
+    constexpr int kPieces = MT * 16 * kRowPieces / (64 * WN);  // pieces a thread stages
+    static_assert(kPieces * 64 * WN == MT * 16 * kRowPieces, "whole pieces");
+    __shared__ __attribute__((aligned(16))) uint8_t xs[2][kStep];
+    __shared__ __attribute__((aligned(16))) uint8_t ws[WN][NT * kTile];
+    constexpr bool kMins = Unit<WT>::kMins;
+    __shared__ __attribute__((aligned(16))) _Float16 gs[kMins ? 2 : 1][kMins ? MT : 1][2][16][8];  // group sums of two units
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 15, j = lane >> 4;
+    const int tiles_b = (a.batch + 16 * MT - 1) / (16 * MT), tiles_n = (a.out_dim + 16 * NT * WN - 1) / (16 * NT * WN);
+    // Workgroups go to the eight XCDs in turn: each XCD gets a run of tiles that share weight rows.
+    const int tiles = tiles_b * tiles_n;
+    const int split = blockIdx.x / tiles;
+    int tile = blockIdx.x % tiles;
+    const int per_xcd = tiles / 8;
+    if (tile < per_xcd * 8) tile = tile % 8 * per_xcd + tile / 8;
+    const int row0 = (tile / tiles_b * WN + wave) * (16 * NT), b0 = tile % tiles_b * (16 * MT);
+    // This split's units of K.
+    const int pairs = a.in_dim >> 6;
+    const int u0 = split * a.units_per_split, u1 = min(u0 + a.units_per_split, (pairs + 3) >> 2);
+
+    // Weights: 16 rows' offsets fit 32 bits.  Rows behind the last are the last again.
+    const auto send = [&](int u) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const int first = min(row0 + 16 * i, a.out_dim - 1), rows = a.out_dim - 1 - first;
+            const uint8_t* base = static_cast<const uint8_t*>(a.w) + (int64_t)first * a.row_bytes + (int64_t)u * kRow;
+            const uint32_t left = (uint32_t)(a.row_bytes - (int64_t)u * kRow - 4);
+            const auto at_byte = [&](int byte) {
+                const int r = byte / kRow;
+                uint32_t col = byte % kRow;
+                if constexpr (!AL) col = min(col, left);
+                return base + (uint64_t)((uint32_t)min(r, rows) * (uint32_t)a.row_bytes + col);
+            };
+            uint8_t* to = &ws[wave][i * kTile];
+            constexpr int kWide = AL ? kTile / 1024 * 1024 : 0;
+#pragma unroll
+            for (int at = 0; at < kWide; at += 1024) load_to_lds<16>(at_byte(at + 16 * lane), to + at);
+#pragma unroll
+            for (int at = kWide; at < kTile; at += 256) load_to_lds<4>(at_byte(at + 4 * lane), to + at);
+        }
+    };
+    // Piece i of a thread: 16 bytes of a row, neighbouring lanes on neighbouring pieces.
+    u4 piece[kPieces];
+    const int b_last = min(16 * MT, a.batch - b0) - 1;
+    const auto fetch_x = [&](int step) {
+        const uint8_t* base = a.x + (int64_t)b0 * a.in_dim;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int p = i * (64 * WN) + (int)threadIdx.x, r = p / kRowPieces;
+            const int c = min(step * (32 * G) + p % kRowPieces * 16, a.in_dim - 16);
+            piece[i] = *reinterpret_cast<const u4*>(base + (uint64_t)((uint32_t)min(r, b_last) * (uint32_t)a.in_dim + c));
+        }
+    };
+    // Half of group g of row r is 8 bytes of each of the four lanes (r, j) of the operand; odd groups' rows are turned by
+    // eight, so that a wave's writes meet all banks.
+    const auto stage_x = [&](int step) {
+        const int buf = step % 2;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int p = i * (64 * WN) + (int)threadIdx.x, r = p / kRowPieces, g = p % kRowPieces / 2, half = p & 1;
+            uint8_t* to = &xs[buf][((r >> 4) * G + g) * 1024 + ((r & 15) ^ (8 * (g & 1))) * 16 + half * 8];
+            float total = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const Terms t = x_terms(piece[i][k], 0u);
+                *reinterpret_cast<u2*>(to + k * 256) = u2{t.r[0], t.r[1]};
+                if constexpr (kMins) {
+                    const h2 one = {1.f16, 1.f16};
+                    total = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, t.r[0]), one, total, false);
+                    total = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, t.r[1]), one, total, false);
+                }
+            }
+            if constexpr (kMins) {
+                total += __shfl_xor(total, 1);  // the group's other half is the next lane's
+                const _Float16 hi = (_Float16)total;
+                gs[step / kSteps % 2][r >> 4][half][r & 15][step % kSteps * G + g] =
+                    half ? (_Float16)(total - (float)hi) : hi;
+            }
+        }
+    };
+    Terms xt[2][MT];
+    const int read_at[2] = {lane * 16, (lane ^ 8) * 16};
+    const auto read_x = [&](int buf, int g) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+            xt[g % 2][m] =
+                __builtin_bit_cast(Terms, *reinterpret_cast<const u4*>(&xs[buf][(m * G + g) * 1024 + read_at[g % 2]]));
+    };
+
+    constexpr bool kWholeBlock = WT == GSP_WTYPE_Q4_K;
+    constexpr int kSets = G * NT;  // of a step, in the order group, 16 weight rows
+    f4 acc[NT][MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[i][m] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    const f4 zero = {0.f, 0.f, 0.f, 0.f};
+    uint32_t mask = kNib;
+    asm volatile("" : "+v"(mask));
+    f4 sum[kWholeBlock ? NT : 2][MT];  // Q4_K: the super-block's sums; else the last two sets'
+    const uint32_t keep = j < 2 ? 0xffffffffu : 0u;
+    Dealt<WT> w[NT];
+    const auto take_w = [&](int u) {  // unit u has landed; the next one is sent for
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        Unit<WT> raw[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) raw[i].read(&ws[wave][i * kTile], n, j);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) w[i].deal(raw[i]);
+    };
+    send(u0);
+    fetch_x(kSteps * u0);
+    stage_x(kSteps * u0);
+    fetch_x(kSteps * u0 + 1);
+    lds_barrier();
+    read_x(0, 0);
+    float sc_last = 0.f;
+    if constexpr (!kWholeBlock) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) sum[1][m] = zero;
+    }
+    for (int u = u0; u < u1; ++u) {
+        take_w(u);
+        Terms q = w[0].operand(0, 0, mask);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            // The other buffer was last read before the barrier below, in the step before.
+            stage_x(kSteps * u + s + 1);
+            fetch_x(min(kSteps * u + s + 2, kSteps * u1 - 1));
+            if (s == 0) {
+                // Behind this step's fetch: loads complete in order, and the next step waits for it.
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (u + 1 < u1) send(u + 1);
+            }
+#pragma unroll
+            for (int k = 0; k < kSets; ++k) {
+                const int g = k / NT, i = k % NT, ug = s * G + g, t = ug / 2, h = ug % 2;
+                const int last_i = (k + kSets - 1) % kSets % NT;
+                if (g == G - 1 && i == 0) lds_barrier();  // the next step's activations are staged, this step's in registers
+                if (i == 0) read_x(g < G - 1 ? s % 2 : (s + 1) % 2, (g + 1) % G);
+                const bool live = AL || 4 * u + t < pairs;
+                float sc = 0.f;
+                if constexpr (!kWholeBlock) sc = live ? w[i].scale(t, h) : 0.f;
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    if constexpr (kWholeBlock) {
+                        sum[i][m] = mfma(xt[g % 2][m], q, ug == 0 ? zero : sum[i][m]);
+                    } else {
+                        sum[k % 2][m] = mfma(xt[g % 2][m], q, zero);
+                    }
+                    if constexpr (!kWholeBlock) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[last_i][m][r] = fmaf(sc_last, sum[(k + 1) % 2][m][r], acc[last_i][m][r]);
+                    }
+                }
+                if (k + 1 < kSets || s + 1 < kSteps) {
+                    const int k2 = (k + 1) % kSets, g2 = (s + (k + 1) / kSets) * G + k2 / NT;
+                    q = w[k2 % NT].operand(g2 / 2, g2 % 2, mask);
+                }
+                sc_last = sc;
+                pin(sc_last);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) pin(acc[last_i][m]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if constexpr (kMins) {
+            Terms ms[MT], mn[NT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) ms[m] = __builtin_bit_cast(Terms, *reinterpret_cast<const u4*>(&gs[u % 2][m][j & 1][n][0]));
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                mn[i] = w[i].minimums(keep);
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                    if (!AL && 4 * u + t >= pairs) mn[i].r[t] = 0;
+            }
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    if constexpr (kWholeBlock) {
+                        const f4 low = mfma(ms[m], mn[i], zero);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            acc[i][m][r] = fmaf(w[i].d, sum[i][m][r], fmaf(-w[i].dmin, low[r], acc[i][m][r]));
+                        pin(acc[i][m]);
+                    } else {
+                        acc[i][m] = mfma(ms[m], mn[i], acc[i][m]);
+                    }
+                }
+            }
+        }
+    }
+    if constexpr (!kWholeBlock) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[NT - 1][m][r] = fmaf(sc_last, sum[1][m][r], acc[NT - 1][m][r]);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load outlives the loop
+    float* y = a.partials ? a.partials + (int64_t)split * a.batch * a.out_dim : a.y;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int b = b0 + 16 * m + 4 * j + r;
+            const float f = a.x_scale[min(b, a.batch - 1)];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const int o = row0 + 16 * i + n;
+                if (b < a.batch && o < a.out_dim) y[(int64_t)b * a.out_dim + o] = acc[i][m][r] * f;
+            }
+        }
+    }
+}
+
+// The splits' sums, in their order.
+__global__ __launch_bounds__(256) void add_splits_kernel(const float* part, float* y, int64_t n, int splits) {
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < n; at += (int64_t)gridDim.x * 256) {
+        float s = part[at];
+        for (int i = 1; i < splits; ++i) s += part[i * n + at];
+        y[at] = s;
+    }
+}
+
+template <int WT, int MT, int NT, int WN, int G>
+hipError_t launch_tile(MatmulFp8Args a, int splits, hipStream_t stream) {
+    const bool aligned = a.in_dim % 256 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
+    const int units = (a.in_dim + 255) / 256;
+    a.units_per_split = (units + splits - 1) / splits;
+    if (splits == 1) a.partials = nullptr;
+    const int64_t tiles_n = ((int64_t)a.out_dim + 16 * NT * WN - 1) / (16 * NT * WN);
+    // A launch holds fewer than 2^32 threads: very large batches take several (and no splits).
+    const int64_t most_rows = std::max<int64_t>(1, (1 << 22) / tiles_n) * (16 * MT);
+    for (int64_t left = a.batch; left > 0; left -= most_rows) {
+        a.batch = (int32_t)std::min(left, most_rows);
+        const uint32_t grid = (uint32_t)(tiles_n * ((a.batch + 16 * MT - 1) / (16 * MT)) * splits);
+        if (aligned)
+            hipLaunchKernelGGL((matmul_fp8_tile_kernel<WT, MT, NT, WN, G, true>), dim3(grid), dim3(64 * WN), 0, stream, a);
+        else
+            hipLaunchKernelGGL((matmul_fp8_tile_kernel<WT, MT, NT, WN, G, false>), dim3(grid), dim3(64 * WN), 0, stream, a);
+        if (splits > 1) {
+            const int64_t n = (int64_t)a.batch * a.out_dim;
+            hipLaunchKernelGGL(add_splits_kernel, dim3((uint32_t)std::min<int64_t>((n + 255) / 256, 2048)), dim3(256), 0,
+                               stream, a.partials, a.y, n, splits);
+        }
+        a.x += (int64_t)a.batch * a.in_dim;
+        a.x_scale += a.batch;
+        a.y += (int64_t)a.batch * a.out_dim;
+    }
+    return hipGetLastError();
+}
+
+// Waves for `units` of K, at most `most`, with the units spread evenly.
+int even_waves(int units, int most) {
+    const int per = (units + most - 1) / most;
+    return (units + per - 1) / per;
+}
+
 template <int WT>
-hipError_t launch_type(const MatmulFp8Args& a, hipStream_t stream) {
-    if (a.batch <= 16) return launch_form<WT, 1, 1>(a, stream);
-    if (a.batch <= 32) return launch_form<WT, 2, 1>(a, stream);
-    return launch_form<WT, 4, 1>(a, stream);
+hipError_t launch_type(const MatmulFp8Args& a, const MatmulFp8Plan& p, hipStream_t stream) {
+    const int units = (a.in_dim + 255) / 256;
+    switch (p.form) {
+        case MatmulFp8Plan::kTile128: return launch_tile<WT, 8, 2, 8, 4>(a, p.splits, stream);
+        case MatmulFp8Plan::kTile64: return launch_tile<WT, 4, 1, 8, 4>(a, p.splits, stream);
+        case MatmulFp8Plan::kTile32: return launch_tile<WT, 2, 1, 4, 4>(a, p.splits, stream);
+        default: break;
+    }
+    if (a.batch <= 16 && a.out_dim > 8192) return launch_form<WT, 1, 2, 8>(a, even_waves(units, 8), stream);
+    if (a.batch <= 16) return launch_form<WT, 1, 1, 16>(a, even_waves(units, 16), stream);
+    if (a.batch <= 32 && a.out_dim <= 8192) return launch_form<WT, 2, 1, 8>(a, even_waves(units, 8), stream);
+    return launch_form<WT, 2, 2, 8>(a, even_waves(units, 8), stream);
 }
 
 }  // namespace
+
+// Which form a product takes: the one whose modelled time is least.  A tile's
+// workgroup takes a time per unit of K that depends on how many share its CU;
+// workgroups run in rounds of what the chip holds; splits of K add the partial
+// sums' traffic and a launch.
+MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, int cus) {
+    MatmulFp8Plan best{};
+    // Tile offsets are 32-bit; a longer K is streamed.
+    if (batch <= 64 || in_dim > (1 << 24)) return best;
+    struct Form {
+        int form, rows, cols;
+        double us[4];   // a unit's time with one to four workgroups on a CU; 0: they do not fit
+        double around;  // a round's time before and behind its units
+    };
+    // Measured on 3584 and 18944 of K, Q4_0, at 65 to 2048 rows.
+    constexpr Form kForms[] = {{MatmulFp8Plan::kTile128, 128, 256, {4.85, 0, 0, 0}, 10},
+                               {MatmulFp8Plan::kTile64, 64, 128, {2.05, 3.7, 0, 0}, 4},
+                               {MatmulFp8Plan::kTile32, 32, 64, {1.33, 1.75, 2.5, 3.25}, 4}};
+    const int units = (in_dim + 255) / 256;
+    double least = 0;
+    for (const Form& f : kForms) {
+        const double tiles = (double)(((int64_t)batch + f.rows - 1) / f.rows) * (((int64_t)out_dim + f.cols - 1) / f.cols);
+        int fit = 4;
+        while (fit > 1 && f.us[fit - 1] == 0) --fit;
+        for (int splits = 1; splits <= 16 && splits * 2 <= std::max(2, units); ++splits) {
+            if (splits > 1 && tiles * splits > (double)cus * fit) break;
+            const int per = (units + splits - 1) / splits;
+            if ((units + per - 1) / per != splits) continue;
+            const double on_cu = std::ceil(tiles * splits / cus);
+            const double full = std::floor(on_cu / fit);
+            const int rest = (int)(on_cu - full * fit);
+            double t = (full * f.us[fit - 1] + (rest ? f.us[rest - 1] : 0)) * per;
+            t += f.around * (fit == 1 ? on_cu : 1);
+            if (splits > 1) t += 3.5 + (double)batch * out_dim * 4 * 2 * splits / 4e6;
+            if (least == 0 || t < least) {
+                least = t;
+                best.form = f.form;
+                best.splits = splits;
+            }
+        }
+    }
+    return best;
+}
 
 int64_t matmul_fp8_row_bytes(int32_t w_type, int32_t in_dim) {
     return (int64_t)(in_dim / 64) * (w_type == GSP_WTYPE_Q4_1 ? 40 : 36);
 }
 
-hipError_t launch_matmul_fp8(int32_t w_type, const MatmulFp8Args& a, hipStream_t stream) {
-    if (w_type == GSP_WTYPE_Q4_0) return launch_type<GSP_WTYPE_Q4_0>(a, stream);
-    if (w_type == GSP_WTYPE_Q4_1) return launch_type<GSP_WTYPE_Q4_1>(a, stream);
-    return launch_type<GSP_WTYPE_Q4_K>(a, stream);
+hipError_t launch_matmul_fp8(int32_t w_type, const MatmulFp8Args& a, const MatmulFp8Plan& plan, hipStream_t stream) {
+    if (w_type == GSP_WTYPE_Q4_0) return launch_type<GSP_WTYPE_Q4_0>(a, plan, stream);
+    if (w_type == GSP_WTYPE_Q4_1) return launch_type<GSP_WTYPE_Q4_1>(a, plan, stream);
+    return launch_type<GSP_WTYPE_Q4_K>(a, plan, stream);
 }
 
 }  // namespace gsp

@@ -1154,7 +1154,16 @@ int gsp_matmul_batch_fp8(gsp_ctx* ctx, int32_t w_type, const void* w_dev, const 
         return gsp::fail(GSP_E_INVALID_ARG, "y overlaps another argument");
     int rc = set_device(ctx);
     if (rc) return rc;
-    return check_hip(gsp::launch_matmul_fp8(w_type, a, ctx->stream), "matmul_fp8 launch");
+    const gsp::MatmulFp8Plan plan = gsp::plan_matmul_fp8(in_dim, out_dim, batch, std::max(1, ctx->num_cus));
+    if (plan.splits > 1) {
+        MatmulNeeds need;
+        MatmulBuffers* ws = nullptr;
+        need.partials = (size_t)plan.splits * batch * out_dim;
+        rc = matmul_workspace(ctx, need, false, &ws);
+        if (rc) return rc;
+        a.partials = ws->partials;
+    }
+    return check_hip(gsp::launch_matmul_fp8(w_type, a, plan, ctx->stream), "matmul_fp8 launch");
 }
 
 // Q8_0 and K-quant products with at least this many outputs (batch x out_dim)

@@ -271,8 +271,9 @@ int gsp_mrope_write_step(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, int32_t n_
 /* (the reference's RMSNorm, FFN gate and MatMulBatch calls,                 */
 /* PagedTransformerRunner.cs:588-603,659).  Codes are OCP e4m3 bytes, one    */
 /* fp32 scale a row: value = scale * code.  All pointers are device          */
-/* pointers; the calls only enqueue one kernel on the context's stream, keep */
-/* no workspace and can be captured.                                         */
+/* pointers, and all work goes on the context's stream.  gsp_rms_norm and    */
+/* gsp_quantize_fp8 keep no workspace and can be captured as they are;       */
+/* gsp_matmul_batch_fp8 says when it may.                                    */
 /* ------------------------------------------------------------------------ */
 
 /* The root-mean-square norm of `rows` rows of `dim` fp32 values, with the
@@ -311,11 +312,16 @@ int gsp_quantize_fp8(gsp_ctx* ctx, int32_t act, int32_t rows, int32_t dim, int64
  * (GSP_WTYPE_Q4_0, 18 bytes: fp16 d, then 16 bytes whose low halves are weights
  * 0 to 15 and whose high halves are 16 to 31, w = d * (q - 8)) and Q4_1
  * (GSP_WTYPE_Q4_1, 20 bytes: fp16 d, fp16 m, the same 16 bytes, w = d * q + m).
- * The product of weights and codes is exact, sums are fp32: no rounding of x or
+ * Products of codes and quants are exact and sums are fp32: no rounding of x or
  * W is added to the codes' own.  in_dim is a multiple of 64 (256 for Q4_K;
  * GSP_E_UNSUPPORTED otherwise, as for other weight types).  Results are the
- * same bit for bit on every call, and a row's do not depend on the other rows
- * of its batch in value, only in the order of their sums. */
+ * same bit for bit on every call of the same sizes, captured or not; the number
+ * of rows may change the order of an output's sums.
+ * Graph capture is as for gsp_matmul_batch: products of more than 64 rows may
+ * need a workspace, so run the product, or a larger one, once before capturing
+ * it (GSP_E_STATE otherwise, and nothing is enqueued); captured products keep
+ * buffers of their own and their graphs must not run at the same time as each
+ * other.  Up to 64 rows nothing is needed. */
 #define GSP_WTYPE_Q4_0 2
 #define GSP_WTYPE_Q4_1 3
 int gsp_matmul_batch_fp8(gsp_ctx* ctx, int32_t w_type, const void* w_dev, const uint8_t* x_dev,

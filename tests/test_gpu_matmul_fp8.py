@@ -17,7 +17,9 @@ TYPES = {"q4_0": Q4_0, "q4_1": Q4_1, "q4_k": Q4_K}
 # (in_dim, out_dim, batch); K-quants skip in_dim that is no multiple of 256.
 SHAPES = [(64, 1, 1), (64, 16, 3), (128, 17, 2), (192, 40, 5), (256, 16, 16), (256, 5, 1), (320, 33, 17), (512, 64, 32),
           (896, 1152, 8), (1024, 100, 33), (3584, 512, 64), (3584, 37, 65), (4864, 896, 1), (18944, 48, 4),
-          (18944, 20, 64), (256, 130, 200), (512, 257, 129), (1280, 96, 300), (64, 300, 1000), (2048, 256, 512)]
+          (18944, 20, 64), (256, 130, 200), (512, 257, 129), (1280, 96, 300), (64, 300, 1000), (2048, 256, 512),
+          # the tile forms: each tile height, with and without ranges of K, ragged ends, K that ends inside a unit
+          (1024, 4000, 65), (4864, 130, 70), (4928, 900, 515), (3584, 3600, 1030), (576, 5000, 1290), (18944, 300, 66)]
 
 
 def _reference(w_type, raw, codes, scale, in_dim):
