@@ -179,8 +179,6 @@ struct MropeWriteArgs {
     int64_t q_stride;
     int64_t k_stride;
     int64_t v_stride;
-    const double* freq;        // as in RopeWriteArgs
-    double log2_base;
     int32_t n;
     int32_t n_heads;
     int32_t n_kv;
@@ -192,6 +190,7 @@ struct MropeWriteArgs {
     int32_t n_axes;
     int32_t interleaved;               // GSP_MROPE_INTERLEAVED
     int32_t sections[kMropeMaxAxes];   // pairs of each axis
+    double rates[kRopeMaxHalf];        // angle per position of each pair
 };
 hipError_t launch_mrope_write(int kv_f16, const MropeWriteArgs& a, hipStream_t stream);
 

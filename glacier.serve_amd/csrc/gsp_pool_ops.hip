@@ -37,6 +37,12 @@ __global__ __launch_bounds__(128) void write_tokens_kernel(WriteTokensArgs a) {
     for (int e = e0 + 256; e < a.v_head_dim; e += 128) vd[e] = static_cast<KT>(vs[e]);
 }
 
+// Pair j's angle: its rate is the table's, or freq_base^(-2j/rope_dim).
+__device__ inline void pair_angle(const RopeWriteArgs& a, double pos, int j, float* c, float* s) {
+    const double rate = a.freq ? a.freq[j] : exp2(-(2.0 * j / a.rope_dim) * a.log2_base);
+    rope_angle(pos, rate, a.mscale, c, s);
+}
+
 // QuantKernels.RoPE then PagedBlockPool.Store for n tokens
 // (PagedTransformerRunner.cs:253-267, 436-449, 619-634), one workgroup per
 // token.  Pair j < rope_dim/2 of every head turns by its angle (Su et al.,
@@ -51,7 +57,7 @@ __global__ __launch_bounds__(256) void rope_write_kernel(RopeWriteArgs a) {
     const int d = a.head_dim;
     const int half = a.rope_dim >> 1;
     const double pos = (double)a.positions[i];
-    for (int j = threadIdx.x; j < half; j += blockDim.x) rope_angle(a, pos, j, &cs[j][0], &cs[j][1]);
+    for (int j = threadIdx.x; j < half; j += blockDim.x) pair_angle(a, pos, j, &cs[j][0], &cs[j][1]);
     __syncthreads();
     const bool stored = a.block_ids[i] >= 0;
     const int64_t dst = (int64_t)a.block_ids[i] * a.block_stride + a.layer_offset + (int64_t)a.slots[i] * d;
@@ -160,7 +166,7 @@ __global__ __launch_bounds__(256) void rope_write_vec_kernel(RopeWriteArgs a) {
     const double pos = (double)a.positions[i];
     const int64_t blk = a.block_ids[i];
     const int64_t slot = a.slots[i];
-    for (int j = threadIdx.x; j < half; j += 256) rope_angle(a, pos, j, &cs[j][0], &cs[j][1]);
+    for (int j = threadIdx.x; j < half; j += 256) pair_angle(a, pos, j, &cs[j][0], &cs[j][1]);
     __syncthreads();
 
     if (kind == 3 || (kind != 0 && blk < 0)) return;

@@ -5,20 +5,17 @@
 
 namespace gsp {
 
-// Cosine and sine of pair j's angle at position `pos`, times the rotation's
-// scale.  The angle, pos times the pair's rate (the table's, or
-// freq_base^(-2j/rope_dim)), is formed and reduced to
-// [-pi, pi] in fp64, so it stays exact at long positions; cosine and sine are
-// fp32.  A scale of 1 leaves them exact.
-template <typename Args>
-__device__ inline void rope_angle(const Args& a, double pos, int j, float* c, float* s) {
-    const double rate = a.freq ? a.freq[j] : exp2(-(2.0 * j / a.rope_dim) * a.log2_base);
+// Cosine and sine of a pair's angle, position times rate, times the rotation's
+// scale.  The angle is formed and reduced to [-pi, pi] in fp64, so it stays
+// exact at long positions; cosine and sine are fp32.  A scale of 1 leaves them
+// exact.
+__device__ inline void rope_angle(double pos, double rate, float mscale, float* c, float* s) {
     const double ang = pos * rate;
     const double r = ang - 6.283185307179586 * rint(ang * 0.15915494309189535);
     float sn, cn;
     sincosf((float)r, &sn, &cn);
-    *c = cn * a.mscale;
-    *s = sn * a.mscale;
+    *c = cn * mscale;
+    *s = sn * mscale;
 }
 
 __device__ inline void rope_turn(float x0, float x1, float c, float s, float* y0, float* y1) {

@@ -161,6 +161,10 @@ struct gsp_ctx {
     std::vector<double> rope_rates[kRopeTables];
     uint64_t rope_used[kRopeTables] = {};
     uint64_t rope_clock = 0;
+    // The rates of the last rotation by formula that gsp_mrope_write_step made.
+    int32_t mrope_dim = 0;
+    float mrope_base = 0.0f;
+    double mrope_rates[gsp::kRopeMaxHalf];
 };
 
 struct gsp_pool {
@@ -702,6 +706,15 @@ int rope_table(gsp_ctx* ctx, const std::vector<double>& rates, const double** ou
     return GSP_OK;
 }
 
+// The angle per position of each pair of a checked rotation.
+void rope_rates(const gsp_rope_spec& spec, const RopeSetup& r, double* rates) {
+    for (int32_t j = 0; j < r.rope_dim / 2; ++j) {
+        double rate = spec.inv_freq ? (double)spec.inv_freq[j] : std::exp2(-(2.0 * j / r.rope_dim) * r.log2_base);
+        if (spec.freq_factors) rate /= (double)spec.freq_factors[j];
+        rates[j] = rate;
+    }
+}
+
 // Checks a rotation against the pool (QuantKernels.RoPE's arguments,
 // PagedTransformerRunner.cs:253-264) and resolves it; with `ctx` (after
 // set_device) it also places its table on the device.
@@ -738,11 +751,7 @@ int check_rope(gsp_ctx* ctx, const gsp_pool* pool, int32_t n_heads, const gsp_ro
     out->log2_base = spec->inv_freq ? 0.0 : std::log2((double)spec->freq_base);
     if (!ctx || (!spec->inv_freq && !spec->freq_factors)) return GSP_OK;
     std::vector<double> rates((size_t)half);
-    for (int32_t j = 0; j < half; ++j) {
-        double r = spec->inv_freq ? (double)spec->inv_freq[j] : std::exp2(-(2.0 * j / rope_dim) * out->log2_base);
-        if (spec->freq_factors) r /= (double)spec->freq_factors[j];
-        rates[j] = r;
-    }
+    rope_rates(*spec, *out, rates.data());
     return rope_table(ctx, rates, &out->freq);
 }
 
@@ -968,7 +977,7 @@ int gsp_rope_write_step(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, int32_t n_h
 
 int gsp_mrope_write_step(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, int32_t n_heads, const gsp_mrope_spec* spec,
                          const int32_t* positions_dev, const float* q_dev, int64_t q_stride, float* q_out_dev,
-                         const float* k_dev, int64_t k_stride, const float* v_dev, int64_t v_stride) try {
+                         const float* k_dev, int64_t k_stride, const float* v_dev, int64_t v_stride) {
     gsp::clear_error();
     int rc = check_write_step(ctx, pool, layer, k_dev, v_dev);
     if (rc) return rc;
@@ -1007,7 +1016,6 @@ int gsp_mrope_write_step(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, int32_t n_
     }
     bool cap = false;
     rc = step_begin(ctx, &cap);
-    if (!rc) rc = check_rope(ctx, pool, n_heads, &spec->rope, q_dev, &r);
     if (rc) return rc;
     const int32_t* wr = ctx->d_step + ctx->off_wr;
     gsp::MropeWriteArgs a{};
@@ -1029,8 +1037,6 @@ int gsp_mrope_write_step(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, int32_t n_
     a.q_stride = q_stride;
     a.k_stride = k_stride;
     a.v_stride = v_stride;
-    a.freq = r.freq;
-    a.log2_base = r.log2_base;
     a.n = n;
     a.n_heads = n_heads;
     a.n_kv = d.heads_kv;
@@ -1039,14 +1045,23 @@ int gsp_mrope_write_step(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, int32_t n_
     a.style = r.style;
     a.rope_dim = r.rope_dim;
     a.mscale = r.mscale;
+    if (spec->rope.inv_freq || spec->rope.freq_factors) {
+        rope_rates(spec->rope, r, a.rates);
+    } else {
+        // The same formula layer after layer: 64 powers are a microsecond of host time a call.
+        if (ctx->mrope_dim != r.rope_dim || ctx->mrope_base != spec->rope.freq_base) {
+            rope_rates(spec->rope, r, ctx->mrope_rates);
+            ctx->mrope_dim = r.rope_dim;
+            ctx->mrope_base = spec->rope.freq_base;
+        }
+        std::copy_n(ctx->mrope_rates, r.rope_dim / 2, a.rates);
+    }
     a.n_axes = spec->n_axes;
     a.interleaved = spec->layout == GSP_MROPE_INTERLEAVED;
     for (int32_t i = 0; i < spec->n_axes; ++i) a.sections[i] = spec->sections[i];
     rc = check_hip(gsp::launch_mrope_write(d.kv_dtype == GSP_KV_F16, a, ctx->stream), "mrope_write launch");
     const int rd = step_done(ctx, cap);
     return rc ? rc : rd;
-} catch (const std::bad_alloc&) {
-    return gsp::fail(GSP_E_OOM, "host memory ran out");
 }
 
 int gsp_rms_norm(gsp_ctx* ctx, int32_t rows, int32_t dim, const float* x_dev, const float* residual_dev,

@@ -653,14 +653,21 @@ class MRope(Rope):
     def __init__(self, freq_base: float, sections: Sequence[int], style: int = 0, layout: int = 0, rope_dim: int = 0,
                  inv_freq=None, freq_factors=None, mscale: float = 0.0):
         super().__init__(freq_base, style, rope_dim, inv_freq, freq_factors, mscale)
-        self.sections = [int(n) for n in sections]
+        self.sections = tuple(int(n) for n in sections)
         self.layout = int(layout)
         if len(self.sections) > MROPE_MAX_AXES:
             raise ValueError(f"{len(self.sections)} axes; at most {MROPE_MAX_AXES}")
 
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        object.__setattr__(self, "_specs", {})  # the C structs made so far, by head_dim
+
     def spec(self, head_dim: int) -> MRopeSpec:
-        return MRopeSpec(super().spec(head_dim), len(self.sections), (i32 * MROPE_MAX_AXES)(*self.sections),
-                         self.layout)
+        spec = self._specs.get(head_dim)
+        if spec is None:
+            spec = self._specs[head_dim] = MRopeSpec(super().spec(head_dim), len(self.sections),
+                                                     (i32 * MROPE_MAX_AXES)(*self.sections), self.layout)
+        return spec
 
 
 def prefix_hash(parent_hash: int, tokens) -> int:

@@ -250,8 +250,9 @@ int gsp_rope_write_step_ex(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, int32_t 
  * fused projection can be given as they lie.  The turned Q goes to q_out_dev,
  * dense [total_q][n_heads][head_dim], which may be q_dev itself if that is
  * dense, and may not overlap any input otherwise (GSP_E_INVALID_ARG).  n_heads
- * 0 leaves Q out.  K and V go where gsp_rope_write_step stores them.  Tables and
- * graph capture are as for gsp_rope_write_step_ex. */
+ * 0 leaves Q out.  K and V go where gsp_rope_write_step stores them.  The tables
+ * travel with the launch: any may be used for the first time while the stream
+ * captures.  Otherwise capture is as for gsp_rope_write_step. */
 #define GSP_MROPE_SECTIONS 0
 #define GSP_MROPE_INTERLEAVED 1
 #define GSP_MROPE_MAX_AXES 4
