@@ -238,6 +238,7 @@ struct MatmulFp8Plan {
     enum { kStream = 0, kTile128, kTile64, kTile32 };
     int32_t form = kStream;
     int32_t splits = 1;
+    int32_t cus = 1;
 };
 MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, int cus);
 int64_t matmul_fp8_row_bytes(int32_t w_type, int32_t in_dim);

@@ -233,29 +233,36 @@ __device__ inline void load_to_lds(const uint8_t* from, uint8_t* to) {
         __builtin_amdgcn_global_load_lds(f, t, 4, 0, 0);
 }
 
-// One workgroup: 16 * NT weight rows by 16 * MT batch rows.  Its waves share
+// One workgroup: 16 * NT weight rows by 4 * R * MT batch rows.  Its waves share
 // the units of K, each with sums of its own, which are added in the order of
 // the waves at the end.
 //
 // Each wave has a slot of LDS for one unit of weights and of activations.  Loads
 // go straight there, with neighbouring lanes on neighbouring bytes: a lane that
 // loaded what it multiplies would put each 16 bytes of an instruction on another
-// row, one cache access a lane.  The wave takes the landed unit into registers
-// and sends the next one's loads off before it computes.  AL: rows of weights are
-// 16-byte aligned and whole units; otherwise they are loaded 4 bytes a lane.
-template <int WT, int MT, int NT, int W, bool AL>
+// row, one cache access a lane.  The wave takes the landed unit into registers and
+// sends for the next one before it computes (a second slot, two units ahead, gained
+// nothing).  AL: rows of weights are 16-byte aligned and whole units; otherwise they
+// are loaded 4 bytes a lane.
+//
+// R of the four sums that a lane has of a product are used: batch row 4 R m + R j + r
+// is row 4 j + r of the m-th operand, so that up to four batch rows (R 1) cost one
+// multiply-add an output tile and group, and their activations a quarter of the slot.
+template <int WT, int MT, int R, int NT, int W, bool AL>
 __global__ __launch_bounds__(64 * W) void matmul_fp8_kernel(MatmulFp8Args a) {
-    constexpr int kRow = Unit<WT>::kRow, kTile = 16 * kRow, kSlot = NT * kTile + MT * 4096;
-    static_assert(W * kSlot >= W * NT * MT * 1024, "the partial sums take the slots' place");
+    constexpr int kRow = Unit<WT>::kRow, kTile = 16 * kRow, kX = 4 * R * 256, kSlot = NT * kTile + MT * kX;
+    constexpr int kWide = AL ? kTile / 1024 * 1024 : 0;  // of a tile, loaded 16 bytes a lane
+    static_assert(kSlot >= NT * MT * R * 256, "the partial sums take the slots' place");
     __shared__ __attribute__((aligned(16))) uint8_t lds[W * kSlot];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int n = lane & 15, j = lane >> 4;
-    const int tiles_b = (a.batch + 16 * MT - 1) / (16 * MT);
-    const int row0 = blockIdx.x / tiles_b * (16 * NT), b0 = blockIdx.x % tiles_b * (16 * MT);
+    const int tiles_b = (a.batch + 4 * R * MT - 1) / (4 * R * MT);
+    const int row0 = blockIdx.x / tiles_b * (16 * NT), b0 = blockIdx.x % tiles_b * (4 * R * MT);
     const int pairs = a.in_dim >> 6, units = (pairs + 3) >> 2;
     uint8_t* slot = lds + wave * kSlot;
 
     // Where a lane's bytes of a tile lie: the tile's LDS image is 16 rows of kRow bytes, filled in the lanes' order.
+    // Bytes past a row's end are its last ones again and meet no product.
     const uint8_t* w0 = static_cast<const uint8_t*>(a.w);
     const auto weight_at = [&](int i, int byte, int u) {
         const int r = byte / kRow, c = byte % kRow;
@@ -264,18 +271,18 @@ __global__ __launch_bounds__(64 * W) void matmul_fp8_kernel(MatmulFp8Args a) {
         if constexpr (!AL) col = min(col, a.row_bytes - 4);
         return w0 + row + col;
     };
-    // Piece p (16 bytes) of row r of activations goes to place p ^ r of the row, so that the reads below spread over
-    // the banks.  Bytes past the row's end are its last piece again and meet no product.
+    // Piece p (16 bytes) of row r of activations goes to place p ^ (4 r and on) of the row, so that the reads below
+    // spread over the banks.
+    const auto turn = [](int r) { return R == 1 ? 4 * r : R == 2 ? 2 * r : r; };
     const auto x_at = [&](int m, int i, int u) {
-        const int r = 4 * i + (lane >> 4), p = (lane & 15) ^ r;
-        const int64_t row = (int64_t)min(b0 + 16 * m + r, a.batch - 1) * a.in_dim;
+        const int r = 4 * i + (lane >> 4), p = (lane & 15) ^ turn(r);
+        const int64_t row = (int64_t)min(b0 + 4 * R * m + r, a.batch - 1) * a.in_dim;
         return a.x + row + min(u * 256 + p * 16, a.in_dim - 16);
     };
     const auto send = [&](int u) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             uint8_t* to = slot + i * kTile;
-            constexpr int kWide = AL ? kTile / 1024 * 1024 : 0;
 #pragma unroll
             for (int at = 0; at < kWide; at += 1024) load_to_lds<16>(weight_at(i, at + 16 * lane, u), to + at);
 #pragma unroll
@@ -284,15 +291,20 @@ __global__ __launch_bounds__(64 * W) void matmul_fp8_kernel(MatmulFp8Args a) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) load_to_lds<16>(x_at(m, i, u), slot + NT * kTile + m * 4096 + i * 1024);
+            for (int i = 0; i < R; ++i) load_to_lds<16>(x_at(m, i, u), slot + NT * kTile + m * kX + i * 1024);
         }
     };
+    // Lane (n, j)'s row of the m-th operand: row n is batch row R (n / 4) + n % 4 where that is below R.
+    const int xr = R * (n >> 2) + min(n & 3, R - 1);
 
-    f4 acc[NT][MT];
+    float acc[NT][MT][R];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[i][m] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int m = 0; m < MT; ++m) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) acc[i][m][r] = 0.f;
+        }
     }
     if (wave < units) send(wave);
     for (int u = wave; u < units; u += waves) {
@@ -305,7 +317,7 @@ __global__ __launch_bounds__(64 * W) void matmul_fp8_kernel(MatmulFp8Args a) {
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
             for (int m = 0; m < MT; ++m)
-                xq[t][m] = *reinterpret_cast<const u4*>(slot + NT * kTile + m * 4096 + n * 256 + ((4 * t + j) ^ n) * 16);
+                xq[t][m] = *reinterpret_cast<const u4*>(slot + NT * kTile + m * kX + xr * 256 + ((4 * t + j) ^ turn(xr)) * 16);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and is in registers: the slot may be overwritten
         if (u + waves < units) send(u + waves);
@@ -339,7 +351,7 @@ __global__ __launch_bounds__(64 * W) void matmul_fp8_kernel(MatmulFp8Args a) {
                     for (int m = 0; m < MT; ++m) {
                         const f4 s = mfma(xt[m], q, Unit<WT>::kMins ? f4{0.f, 0.f, 0.f, 0.f} : sx[m]);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
+                        for (int r = 0; r < R; ++r) {
                             acc[i][m][r] = fmaf(sc, s[r], acc[i][m][r]);
                             if constexpr (Unit<WT>::kMins) acc[i][m][r] = fmaf(mn, sx[m][r], acc[i][m][r]);
                         }
@@ -348,41 +360,45 @@ __global__ __launch_bounds__(64 * W) void matmul_fp8_kernel(MatmulFp8Args a) {
             }
         }
     }
-    __syncthreads();  // every wave is done with its slot
-    float* part = reinterpret_cast<float*>(lds);  // [waves][NT][MT][256]
-    // Lane (n, j) holds batch rows 4j .. 4j + 3 of weight row n.
+    __syncthreads();  // every wave is done with its slots
+    float* part = reinterpret_cast<float*>(lds);  // [waves][NT][MT][4 R][16]
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                part[((wave * NT + i) * MT + m) * 256 + (4 * j + r) * 16 + n] = acc[i][m][r];
+            for (int r = 0; r < R; ++r) part[(((wave * NT + i) * MT + m) * 4 * R + R * j + r) * 16 + n] = acc[i][m][r];
         }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < NT * MT * 256; e += blockDim.x) {
+    for (int e = threadIdx.x; e < NT * MT * R * 64; e += blockDim.x) {
         float s = 0.f;
-        for (int v = 0; v < waves; ++v) s += part[v * (NT * MT * 256) + e];
-        const int i = e / (MT * 256), m = e / 256 % MT;
-        const int b = b0 + 16 * m + (e >> 4) % 16, o = row0 + 16 * i + (e & 15);
+        for (int v = 0; v < waves; ++v) s += part[v * (NT * MT * R * 64) + e];
+        const int i = e / (MT * R * 64), b = b0 + e / 16 % (MT * R * 4), o = row0 + 16 * i + (e & 15);
         if (b < a.batch && o < a.out_dim) a.y[(int64_t)b * a.out_dim + o] = s * kCode * a.x_scale[b];
     }
 }
 
-template <int WT, int MT, int NT, int W>
-hipError_t launch_form(MatmulFp8Args a, int waves, hipStream_t stream) {
+// Waves for `units` of K, at most `most`, with the units spread evenly.
+int even_waves(int units, int most) {
+    const int per = (units + most - 1) / most;
+    return (units + per - 1) / per;
+}
+
+template <int WT, int MT, int R, int NT, int W>
+hipError_t launch_form(MatmulFp8Args a, hipStream_t stream) {
+    const int waves = even_waves((a.in_dim + 255) / 256, W);
     const bool aligned = a.in_dim % 256 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
     // A launch holds fewer than 2^32 threads: very large batches take several.
     const int64_t tiles = ((int64_t)a.out_dim + 16 * NT - 1) / (16 * NT);
-    const int64_t most_rows = std::max<int64_t>(1, (1 << 21) / tiles) * (16 * MT);
+    const int64_t most_rows = std::max<int64_t>(1, (1 << 21) / tiles) * (4 * R * MT);
     for (int64_t left = a.batch; left > 0; left -= most_rows) {
         a.batch = (int32_t)std::min(left, most_rows);
-        const uint32_t grid = (uint32_t)(tiles * ((a.batch + 16 * MT - 1) / (16 * MT)));
+        const uint32_t grid = (uint32_t)(tiles * ((a.batch + 4 * R * MT - 1) / (4 * R * MT)));
         if (aligned)
-            hipLaunchKernelGGL((matmul_fp8_kernel<WT, MT, NT, W, true>), dim3(grid), dim3(64 * waves), 0, stream, a);
+            hipLaunchKernelGGL((matmul_fp8_kernel<WT, MT, R, NT, W, true>), dim3(grid), dim3(64 * waves), 0, stream, a);
         else
-            hipLaunchKernelGGL((matmul_fp8_kernel<WT, MT, NT, W, false>), dim3(grid), dim3(64 * waves), 0, stream, a);
+            hipLaunchKernelGGL((matmul_fp8_kernel<WT, MT, R, NT, W, false>), dim3(grid), dim3(64 * waves), 0, stream, a);
         a.x += (int64_t)a.batch * a.in_dim;
         a.x_scale += a.batch;
         a.y += (int64_t)a.batch * a.out_dim;
@@ -676,25 +692,31 @@ hipError_t launch_tile(MatmulFp8Args a, int splits, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// Waves for `units` of K, at most `most`, with the units spread evenly.
-int even_waves(int units, int most) {
-    const int per = (units + most - 1) / most;
-    return (units + per - 1) / per;
-}
-
 template <int WT>
 hipError_t launch_type(const MatmulFp8Args& a, const MatmulFp8Plan& p, hipStream_t stream) {
-    const int units = (a.in_dim + 255) / 256;
     switch (p.form) {
         case MatmulFp8Plan::kTile128: return launch_tile<WT, 8, 2, 8, 4>(a, p.splits, stream);
         case MatmulFp8Plan::kTile64: return launch_tile<WT, 4, 1, 8, 4>(a, p.splits, stream);
         case MatmulFp8Plan::kTile32: return launch_tile<WT, 2, 1, 4, 4>(a, p.splits, stream);
         default: break;
     }
-    if (a.batch <= 16 && a.out_dim > 8192) return launch_form<WT, 1, 2, 8>(a, even_waves(units, 8), stream);
-    if (a.batch <= 16) return launch_form<WT, 1, 1, 16>(a, even_waves(units, 16), stream);
-    if (a.batch <= 32 && a.out_dim <= 8192) return launch_form<WT, 2, 1, 8>(a, even_waves(units, 8), stream);
-    return launch_form<WT, 2, 2, 8>(a, even_waves(units, 8), stream);
+    // The stream form.  With many outputs two tiles share a workgroup's activations; with few, more waves share a tile's
+    // K.  us, Q4_0: 4096 x 14336 at 1 row 9.6 with two tiles and 4 waves, 12.8 with one tile and 16; 3584 x 4608 6.3 and
+    // 6.9; 18944 x 3584 at 1 row 10.7 with one tile and 16 waves, 15 with two tiles.
+    const bool wide = a.out_dim > 4096;
+    if (a.batch <= 4)
+        return wide ? launch_form<WT, 1, 1, 2, 4>(a, stream) : launch_form<WT, 1, 1, 1, 16>(a, stream);
+    if (a.batch <= 8)
+        return wide ? launch_form<WT, 1, 2, 2, 8>(a, stream) : launch_form<WT, 1, 2, 1, 16>(a, stream);
+    if (a.batch <= 16)
+        return wide ? launch_form<WT, 1, 4, 2, 8>(a, stream) : launch_form<WT, 1, 4, 1, 8>(a, stream);
+    // More rows: 32 a workgroup while its workgroups, one a CU, run in one round (18944 x 3584 at 32 rows 19.5 us with
+    // one tile; at 64 rows 27.6 with two); else 16 a workgroup (3584 x 4608 at 37 rows 10.2, 13 with 32).
+    const int64_t tiles_b = (a.batch + 31) / 32;
+    if (a.out_dim >= 16384 && a.batch <= 32) return launch_form<WT, 2, 4, 2, 4>(a, stream);
+    if ((a.out_dim + 15) / 16 * tiles_b <= p.cus) return launch_form<WT, 2, 4, 1, 8>(a, stream);
+    if ((a.out_dim + 31) / 32 * tiles_b <= p.cus) return launch_form<WT, 2, 4, 2, 8>(a, stream);
+    return launch_form<WT, 1, 4, 2, 8>(a, stream);
 }
 
 }  // namespace
@@ -705,8 +727,9 @@ hipError_t launch_type(const MatmulFp8Args& a, const MatmulFp8Plan& p, hipStream
 // sums' traffic and a launch.
 MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, int cus) {
     MatmulFp8Plan best{};
-    // Tile offsets are 32-bit; a longer K is streamed.
-    if (batch <= 64 || in_dim > (1 << 24)) return best;
+    best.cus = cus;
+    // Tile offsets are 32-bit; a longer K is streamed.  Up to 64 rows only wide outputs repay the conversion.
+    if (in_dim > (1 << 24) || batch <= (out_dim >= 16384 ? 32 : 64)) return best;
     struct Form {
         int form, rows, cols;
         double us[4];   // a unit's time with one to four workgroups on a CU; 0: they do not fit
@@ -722,7 +745,7 @@ MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, in
         const double tiles = (double)(((int64_t)batch + f.rows - 1) / f.rows) * (((int64_t)out_dim + f.cols - 1) / f.cols);
         int fit = 4;
         while (fit > 1 && f.us[fit - 1] == 0) --fit;
-        for (int splits = 1; splits <= 16 && splits * 2 <= std::max(2, units); ++splits) {
+        for (int splits = 1; splits <= (batch > 64 ? 16 : 1) && splits * 2 <= std::max(2, units); ++splits) {
             if (splits > 1 && tiles * splits > (double)cus * fit) break;
             const int per = (units + splits - 1) / splits;
             if ((units + per - 1) / per != splits) continue;
