@@ -227,6 +227,8 @@ struct MatmulFp8Args {
     const float* x_scale;  // [batch]
     float* y;              // [batch][out_dim]
     float* partials;       // [splits][batch][out_dim] with several splits of K, else null
+    uint8_t* xf;           // matmul_fp8_x_bytes for converted activations, or null where that is 0
+    uint8_t* sums;         // their group sums, within xf; launch_matmul_fp8 sets it
     int64_t row_bytes;
     int32_t units_per_split;  // 256 of K each; launch_matmul_fp8 sets it
     int32_t in_dim;        // a multiple of 64 (Q4_K: of 256)
@@ -241,6 +243,7 @@ struct MatmulFp8Plan {
     int32_t cus = 1;
 };
 MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, int cus);
+int64_t matmul_fp8_x_bytes(int32_t in_dim, int32_t batch, const MatmulFp8Plan& plan);
 int64_t matmul_fp8_row_bytes(int32_t w_type, int32_t in_dim);
 hipError_t launch_matmul_fp8(int32_t w_type, const MatmulFp8Args& a, const MatmulFp8Plan& plan, hipStream_t stream);
 

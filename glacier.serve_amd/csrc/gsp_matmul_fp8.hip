@@ -419,29 +419,39 @@ __device__ inline void lds_barrier() {
 }
 
 // The tile form, for batches that use an expanded weight many times: 16 * MT
-// batch rows by 16 * NT * WN weight rows a workgroup.  Activations are converted
-// once a workgroup into LDS, in the order the instruction's operands take, 128 of K
-// at a time in two buffers; each wave has its own weight rows, in a slot as above.
+// batch rows by 16 * NT * WN weight rows a workgroup.  Activations lie in LDS as
+// fp16, in the order the instruction's operands take, 32 G of K at a time in two
+// buffers: each workgroup converts its own (PRE false), or they come converted from
+// matmul_fp8_convert_kernel (PRE), which pays for its launch where many workgroups
+// share rows (3584 x 18944 at 2048 rows: 361 -> 345 us).  Each wave has its own
+// weight rows, in a slot as above.
 //
 // The matrix and the vector units work beside each other: while the products of one
 // set (16 weight rows, all batch rows, one group) run, the previous set's sums are
 // scaled into the outputs' (Q4_0 and Q4_1: one fused multiply-add an output and group
-// is the vector unit's main work) and the next set's weights are expanded.  Q4_1's
-// minimum is a second product straight into the outputs' sums; Q4_K's scales are
-// integers within the operand, so that its sums and those of its minimums run over
-// the eight groups of a super-block in the matrix unit alone.
-template <int WT, int MT, int NT, int WN, int G, bool AL>
+// is the vector unit's main work) and the next set's weights are expanded.  Q4_K's
+// scales are integers within the operand, so that its sums run over the eight groups
+// of a super-block in the matrix unit alone.  Minimums meet the sums of x in one more
+// product a unit: staging adds up each group, and leaves its sum as two fp16 numbers,
+// the nearest and what that leaves (22 bits; a sum has up to 23).
+template <int WT, int MT, int NT, int WN, int G, bool PRE, bool AL>
 __global__ __launch_bounds__(64 * WN) void matmul_fp8_tile_kernel(MatmulFp8Args a) {
     constexpr int kRow = Unit<WT>::kRow, kTile = 16 * kRow;
     constexpr int kSteps = 8 / G;                            // of a unit, G groups of 32 each
     constexpr int kStep = MT * G * 1024;                     // LDS bytes of a step's activations
     constexpr int kRowPieces = 2 * G;                        // 16-byte pieces of a row in a step
     constexpr int kPieces = MT * 16 * kRowPieces / (64 * WN);  // pieces a thread stages
-    static_assert(kPieces * 64 * WN == MT * 16 * kRowPieces, "whole pieces");
-    __shared__ __attribute__((aligned(16))) uint8_t xs[2][kStep];
+    constexpr int kBlocks = MT * G / WN;                       // KB that a wave loads of a converted step
+    static_assert(kPieces * 64 * WN == MT * 16 * kRowPieces && (!PRE || (kBlocks * WN == MT * G && MT == WN)), "even shares");
+    static_assert(!PRE || kSteps == 2, "the waits count a unit of two steps");
+    // Two arrays, so that the compiler sees that loads into one do not concern reads of the other.
+    __shared__ __attribute__((aligned(16))) uint8_t xs0[kStep];
+    __shared__ __attribute__((aligned(16))) uint8_t xs1[kStep];
+    const auto x_buf = [&](int step) { return step % 2 ? xs1 : xs0; };
     __shared__ __attribute__((aligned(16))) uint8_t ws[WN][NT * kTile];
     constexpr bool kMins = Unit<WT>::kMins;
     __shared__ __attribute__((aligned(16))) _Float16 gs[kMins ? 2 : 1][kMins ? MT : 1][2][16][8];  // group sums of two units
+    __shared__ __attribute__((aligned(16))) float scales[16 * MT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, j = lane >> 4;
     const int tiles_b = (a.batch + 16 * MT - 1) / (16 * MT), tiles_n = (a.out_dim + 16 * NT * WN - 1) / (16 * NT * WN);
@@ -454,7 +464,7 @@ __global__ __launch_bounds__(64 * WN) void matmul_fp8_tile_kernel(MatmulFp8Args 
     const int row0 = (tile / tiles_b * WN + wave) * (16 * NT), b0 = tile % tiles_b * (16 * MT);
     // This split's units of K.
     const int pairs = a.in_dim >> 6;
-    const int u0 = split * a.units_per_split, u1 = min(u0 + a.units_per_split, (pairs + 3) >> 2);
+    const int units = (pairs + 3) >> 2, u0 = split * a.units_per_split, u1 = min(u0 + a.units_per_split, units);
 
     // Weights: 16 rows' offsets fit 32 bits.  Rows behind the last are the last again.
     const auto send = [&](int u) {
@@ -477,6 +487,23 @@ __global__ __launch_bounds__(64 * WN) void matmul_fp8_tile_kernel(MatmulFp8Args 
             for (int at = kWide; at < kTile; at += 256) load_to_lds<4>(at_byte(at + 4 * lane), to + at);
         }
     };
+    // Loads of a unit's weights, which the wait below counts.
+    constexpr int kWide16 = AL ? kTile / 1024 : 0;
+    constexpr int kSent = NT * (kWide16 + (kTile - 1024 * kWide16) / 256);
+    // Converted activations (PRE): a step's KB of 16 rows and a group each, and a unit's group sums, a tile a wave.
+    const auto send_x = [&](int step, uint8_t* to) {
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            const int kb = wave * kBlocks + i, m = kb / G, g = kb % G;
+            const int64_t at = ((int64_t)(b0 / 16 + m) * units * 8 + step * G + g) * 1024;
+            load_to_lds<16>(a.xf + at + 16 * lane, to + kb * 1024);
+        }
+    };
+    const auto send_sums = [&](int u) {
+        if (lane < 32)
+            load_to_lds<16>(a.sums + ((int64_t)(b0 / 16 + wave) * units + u) * 512 + 16 * lane,
+                            reinterpret_cast<uint8_t*>(&gs[u % 2][kMins ? wave : 0][0][0][0]));
+    };
     // Piece i of a thread: 16 bytes of a row, neighbouring lanes on neighbouring pieces.
     u4 piece[kPieces];
     const int b_last = min(16 * MT, a.batch - b0) - 1;
@@ -491,12 +518,11 @@ __global__ __launch_bounds__(64 * WN) void matmul_fp8_tile_kernel(MatmulFp8Args 
     };
     // Half of group g of row r is 8 bytes of each of the four lanes (r, j) of the operand; odd groups' rows are turned by
     // eight, so that a wave's writes meet all banks.
-    const auto stage_x = [&](int step) {
-        const int buf = step % 2;
+    const auto stage_x = [&](int step, uint8_t* buf) {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const int p = i * (64 * WN) + (int)threadIdx.x, r = p / kRowPieces, g = p % kRowPieces / 2, half = p & 1;
-            uint8_t* to = &xs[buf][((r >> 4) * G + g) * 1024 + ((r & 15) ^ (8 * (g & 1))) * 16 + half * 8];
+            uint8_t* to = buf + ((r >> 4) * G + g) * 1024 + ((r & 15) ^ (8 * (g & 1))) * 16 + half * 8;
             float total = 0.f;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -517,12 +543,12 @@ __global__ __launch_bounds__(64 * WN) void matmul_fp8_tile_kernel(MatmulFp8Args 
         }
     };
     Terms xt[2][MT];
-    const int read_at[2] = {lane * 16, (lane ^ 8) * 16};
-    const auto read_x = [&](int buf, int g) {
+    const int read_at[2] = {lane * 16, (PRE ? lane : lane ^ 8) * 16};
+    const auto read_x = [&](const uint8_t* buf, int g) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
             xt[g % 2][m] =
-                __builtin_bit_cast(Terms, *reinterpret_cast<const u4*>(&xs[buf][(m * G + g) * 1024 + read_at[g % 2]]));
+                __builtin_bit_cast(Terms, *reinterpret_cast<const u4*>(buf + (m * G + g) * 1024 + read_at[g % 2]));
     };
 
     constexpr bool kWholeBlock = WT == GSP_WTYPE_Q4_K;
@@ -548,11 +574,18 @@ __global__ __launch_bounds__(64 * WN) void matmul_fp8_tile_kernel(MatmulFp8Args 
         for (int i = 0; i < NT; ++i) w[i].deal(raw[i]);
     };
     send(u0);
-    fetch_x(kSteps * u0);
-    stage_x(kSteps * u0);
-    fetch_x(kSteps * u0 + 1);
+    if (threadIdx.x < 16 * MT) scales[threadIdx.x] = a.x_scale[min(b0 + (int)threadIdx.x, a.batch - 1)];
+    if constexpr (PRE) {
+        if constexpr (kMins) send_sums(u0);
+        send_x(kSteps * u0, x_buf(0));
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    } else {
+        fetch_x(kSteps * u0);
+        stage_x(kSteps * u0, x_buf(0));
+        fetch_x(kSteps * u0 + 1);
+    }
     lds_barrier();
-    read_x(0, 0);
+    read_x(x_buf(0), 0);
     float sc_last = 0.f;
     if constexpr (!kWholeBlock) {
 #pragma unroll
@@ -563,20 +596,32 @@ __global__ __launch_bounds__(64 * WN) void matmul_fp8_tile_kernel(MatmulFp8Args 
         Terms q = w[0].operand(0, 0, mask);
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            // The other buffer was last read before the barrier below, in the step before.
-            stage_x(kSteps * u + s + 1);
-            fetch_x(min(kSteps * u + s + 2, kSteps * u1 - 1));
+            // The buffer written here was last read before the barrier below, in the step before.  At the end the last
+            // step and unit are loaded again, for nobody, so that the waits' counts hold.
+            const int last_step = kSteps * u1 - 1;
+            if constexpr (PRE) {
+                send_x(min(kSteps * u + s + 1, last_step), x_buf(s + 1));
+            } else {
+                stage_x(kSteps * u + s + 1, x_buf(s + 1));
+                fetch_x(min(kSteps * u + s + 2, last_step));
+            }
             if (s == 0) {
-                // Behind this step's fetch: loads complete in order, and the next step waits for it.
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                if (u + 1 < u1) send(u + 1);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the unit's weights are in registers
+                send(min(u + 1, u1 - 1));
             }
 #pragma unroll
             for (int k = 0; k < kSets; ++k) {
                 const int g = k / NT, i = k % NT, ug = s * G + g, t = ug / 2, h = ug % 2;
                 const int last_i = (k + kSets - 1) % kSets % NT;
-                if (g == G - 1 && i == 0) lds_barrier();  // the next step's activations are staged, this step's in registers
-                if (i == 0) read_x(g < G - 1 ? s % 2 : (s + 1) % 2, (g + 1) % G);
+                if (g == G - 1 && i == 0) {
+                    // The next step's activations are staged, this step's in registers.  PRE: loads complete in order, and
+                    // behind the next step's only the next unit's weights were sent for, in a unit's first step.
+                    if constexpr (PRE) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(s == 0 ? kSent : 0) : "memory");
+                    lds_barrier();
+                    if constexpr (PRE && kMins)
+                        if (s == 0) send_sums(min(u + 1, u1 - 1));  // every wave is past the sums of the unit before
+                }
+                if (i == 0) read_x(x_buf(g < G - 1 ? s : s + 1), (g + 1) % G);
                 const bool live = AL || 4 * u + t < pairs;
                 float sc = 0.f;
                 if constexpr (!kWholeBlock) sc = live ? w[i].scale(t, h) : 0.f;
@@ -640,18 +685,53 @@ __global__ __launch_bounds__(64 * WN) void matmul_fp8_tile_kernel(MatmulFp8Args 
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load outlives the loop
     float* y = a.partials ? a.partials + (int64_t)split * a.batch * a.out_dim : a.y;
+    const bool whole = b0 + 16 * MT <= a.batch && row0 + 16 * NT <= a.out_dim;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
+        const f4 f = *reinterpret_cast<const f4*>(&scales[16 * m + 4 * j]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int b = b0 + 16 * m + 4 * j + r;
-            const float f = a.x_scale[min(b, a.batch - 1)];
+            float* to = y + (int64_t)b * a.out_dim + row0 + n;
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const int o = row0 + 16 * i + n;
-                if (b < a.batch && o < a.out_dim) y[(int64_t)b * a.out_dim + o] = acc[i][m][r] * f;
-            }
+            for (int i = 0; i < NT; ++i)
+                if (whole || (b < a.batch && row0 + 16 * i + n < a.out_dim)) to[16 * i] = acc[i][m][r] * f[r];
         }
+    }
+}
+
+// Activations for the tile form whose workgroups are many enough that converting
+// them once before pays for a launch: fp16 in the operand's order, [16 rows][group]
+// of 1 KB, lane (row, j)'s 16 bytes behind each other, and each group's sum as two
+// fp16 numbers, [16 rows][unit][2][row][group].  Rows and groups past the end are 0.
+// A thread converts one group of a row.
+__global__ __launch_bounds__(128) void matmul_fp8_convert_kernel(const uint8_t* x, uint8_t* xf, _Float16* sums, int in_dim,
+                                                                 int batch, int units) {
+    const int n = threadIdx.x & 15, g = threadIdx.x >> 4;
+    const int64_t tile = blockIdx.x / units;
+    const int u = blockIdx.x % units;
+    const int64_t row = tile * 16 + n;
+    const int k = u * 256 + g * 32;
+    u4 lo = {0, 0, 0, 0}, hi = lo;
+    if (row < batch && k < in_dim) {
+        const uint8_t* p = x + row * in_dim + k;
+        lo = *reinterpret_cast<const u4*>(p);
+        hi = *reinterpret_cast<const u4*>(p + 16);
+    }
+    uint8_t* to = xf + ((tile * units + u) * 8 + g) * 1024 + n * 16;
+    float total = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const Terms t = x_terms(lo[j], hi[j]);
+        *reinterpret_cast<u4*>(to + j * 256) = __builtin_bit_cast(u4, t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            total = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, t.r[i]), h2{1.f16, 1.f16}, total, false);
+    }
+    if (sums) {
+        _Float16* s = sums + (tile * units + u) * 256 + n * 8 + g;
+        s[0] = (_Float16)total;
+        s[128] = (_Float16)(total - (float)s[0]);
     }
 }
 
@@ -664,7 +744,7 @@ __global__ __launch_bounds__(256) void add_splits_kernel(const float* part, floa
     }
 }
 
-template <int WT, int MT, int NT, int WN, int G>
+template <int WT, int MT, int NT, int WN, int G, bool PRE>
 hipError_t launch_tile(MatmulFp8Args a, int splits, hipStream_t stream) {
     const bool aligned = a.in_dim % 256 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
     const int units = (a.in_dim + 255) / 256;
@@ -672,14 +752,20 @@ hipError_t launch_tile(MatmulFp8Args a, int splits, hipStream_t stream) {
     if (splits == 1) a.partials = nullptr;
     const int64_t tiles_n = ((int64_t)a.out_dim + 16 * NT * WN - 1) / (16 * NT * WN);
     // A launch holds fewer than 2^32 threads: very large batches take several (and no splits).
-    const int64_t most_rows = std::max<int64_t>(1, (1 << 22) / tiles_n) * (16 * MT);
+    const int64_t most_rows = std::max<int64_t>(1, (1 << 22) / std::max<int64_t>(tiles_n, PRE ? units : 1)) * (16 * MT);
     for (int64_t left = a.batch; left > 0; left -= most_rows) {
         a.batch = (int32_t)std::min(left, most_rows);
+        if constexpr (PRE) {
+            const int64_t row_tiles = (a.batch + 16 * MT - 1) / (16 * MT) * MT;
+            a.sums = Unit<WT>::kMins ? a.xf + row_tiles * units * 8192 : nullptr;
+            hipLaunchKernelGGL(matmul_fp8_convert_kernel, dim3((uint32_t)(row_tiles * units)), dim3(128), 0, stream, a.x, a.xf,
+                               reinterpret_cast<_Float16*>(a.sums), a.in_dim, a.batch, units);
+        }
         const uint32_t grid = (uint32_t)(tiles_n * ((a.batch + 16 * MT - 1) / (16 * MT)) * splits);
         if (aligned)
-            hipLaunchKernelGGL((matmul_fp8_tile_kernel<WT, MT, NT, WN, G, true>), dim3(grid), dim3(64 * WN), 0, stream, a);
+            hipLaunchKernelGGL((matmul_fp8_tile_kernel<WT, MT, NT, WN, G, PRE, true>), dim3(grid), dim3(64 * WN), 0, stream, a);
         else
-            hipLaunchKernelGGL((matmul_fp8_tile_kernel<WT, MT, NT, WN, G, false>), dim3(grid), dim3(64 * WN), 0, stream, a);
+            hipLaunchKernelGGL((matmul_fp8_tile_kernel<WT, MT, NT, WN, G, PRE, false>), dim3(grid), dim3(64 * WN), 0, stream, a);
         if (splits > 1) {
             const int64_t n = (int64_t)a.batch * a.out_dim;
             hipLaunchKernelGGL(add_splits_kernel, dim3((uint32_t)std::min<int64_t>((n + 255) / 256, 2048)), dim3(256), 0,
@@ -695,9 +781,9 @@ hipError_t launch_tile(MatmulFp8Args a, int splits, hipStream_t stream) {
 template <int WT>
 hipError_t launch_type(const MatmulFp8Args& a, const MatmulFp8Plan& p, hipStream_t stream) {
     switch (p.form) {
-        case MatmulFp8Plan::kTile128: return launch_tile<WT, 8, 2, 8, 4>(a, p.splits, stream);
-        case MatmulFp8Plan::kTile64: return launch_tile<WT, 4, 1, 8, 4>(a, p.splits, stream);
-        case MatmulFp8Plan::kTile32: return launch_tile<WT, 2, 1, 4, 4>(a, p.splits, stream);
+        case MatmulFp8Plan::kTile128: return launch_tile<WT, 8, 2, 8, 4, true>(a, p.splits, stream);
+        case MatmulFp8Plan::kTile64: return launch_tile<WT, 4, 1, 8, 4, false>(a, p.splits, stream);
+        case MatmulFp8Plan::kTile32: return launch_tile<WT, 2, 1, 4, 4, false>(a, p.splits, stream);
         default: break;
     }
     // The stream form.  With many outputs two tiles share a workgroup's activations; with few, more waves share a tile's
@@ -763,6 +849,11 @@ MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, in
         }
     }
     return best;
+}
+
+int64_t matmul_fp8_x_bytes(int32_t in_dim, int32_t batch, const MatmulFp8Plan& plan) {
+    // 16 rows of a unit: 8 KB of activations, 512 bytes of sums.
+    return plan.form == MatmulFp8Plan::kTile128 ? ((int64_t)batch + 127) / 128 * 8 * ((in_dim + 255) / 256) * (8192 + 512) : 0;
 }
 
 int64_t matmul_fp8_row_bytes(int32_t w_type, int32_t in_dim) {

@@ -1170,13 +1170,15 @@ int gsp_matmul_batch_fp8(gsp_ctx* ctx, int32_t w_type, const void* w_dev, const 
     int rc = set_device(ctx);
     if (rc) return rc;
     const gsp::MatmulFp8Plan plan = gsp::plan_matmul_fp8(in_dim, out_dim, batch, std::max(1, ctx->num_cus));
-    if (plan.splits > 1) {
-        MatmulNeeds need;
+    MatmulNeeds need;
+    if (plan.splits > 1) need.partials = (size_t)plan.splits * batch * out_dim;
+    need.x = (size_t)gsp::matmul_fp8_x_bytes(in_dim, batch, plan) / sizeof(uint16_t);
+    if (need.partials || need.x) {
         MatmulBuffers* ws = nullptr;
-        need.partials = (size_t)plan.splits * batch * out_dim;
         rc = matmul_workspace(ctx, need, false, &ws);
         if (rc) return rc;
         a.partials = ws->partials;
+        a.xf = reinterpret_cast<uint8_t*>(ws->x);
     }
     return check_hip(gsp::launch_matmul_fp8(w_type, a, plan, ctx->stream), "matmul_fp8 launch");
 }
