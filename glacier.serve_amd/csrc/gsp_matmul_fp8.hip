@@ -752,7 +752,7 @@ hipError_t launch_tile(MatmulFp8Args a, int splits, hipStream_t stream) {
     if (splits == 1) a.partials = nullptr;
     const int64_t tiles_n = ((int64_t)a.out_dim + 16 * NT * WN - 1) / (16 * NT * WN);
     // A launch holds fewer than 2^32 threads: very large batches take several (and no splits).
-    const int64_t most_rows = std::max<int64_t>(1, (1 << 22) / std::max<int64_t>(tiles_n, PRE ? units : 1)) * (16 * MT);
+    const int64_t most_rows = std::max<int64_t>(1, (1 << 21) / std::max<int64_t>(tiles_n, PRE ? units : 1)) * (16 * MT);
     for (int64_t left = a.batch; left > 0; left -= most_rows) {
         a.batch = (int32_t)std::min(left, most_rows);
         if constexpr (PRE) {

@@ -1152,6 +1152,8 @@ int gsp_matmul_batch_fp8(gsp_ctx* ctx, int32_t w_type, const void* w_dev, const 
     if (in_dim == 0 || in_dim % unit != 0)
         return gsp::fail(GSP_E_UNSUPPORTED, "inDim must be a positive multiple of %d for weight type %d (got %d)", unit,
                          w_type, in_dim);
+    if (out_dim > (1 << 24))
+        return gsp::fail(GSP_E_UNSUPPORTED, "outDim %d: one product has at most %d outputs a row", out_dim, 1 << 24);
     if (!is_aligned(w_dev, 4) || !is_aligned(x_dev, 16) || !is_aligned(x_scale_dev, 4) || !is_aligned(y_dev, 4))
         return gsp::fail(GSP_E_INVALID_ARG, "weights must be 4-byte aligned, x 16-byte aligned, scales and y 4-byte aligned");
     gsp::MatmulFp8Args a{};

@@ -314,9 +314,9 @@ int gsp_quantize_fp8(gsp_ctx* ctx, int32_t act, int32_t rows, int32_t dim, int64
  * 0 to 15 and whose high halves are 16 to 31, w = d * (q - 8)) and Q4_1
  * (GSP_WTYPE_Q4_1, 20 bytes: fp16 d, fp16 m, the same 16 bytes, w = d * q + m).
  * Products of codes and quants are exact and sums are fp32: no rounding of x or
- * W is added to the codes' own.  in_dim is a multiple of 64 (256 for Q4_K;
- * GSP_E_UNSUPPORTED otherwise, as for other weight types).  Results are the
- * same bit for bit on every call of the same sizes, captured or not; the number
+ * W is added to the codes' own.  in_dim is a multiple of 64 (256 for Q4_K)
+ * and out_dim at most 2^24 (GSP_E_UNSUPPORTED otherwise, as for other weight
+ * types).  Results are the same bit for bit on every call of the same sizes, captured or not; the number
  * of rows may change the order of an output's sums.
  * Graph capture is as for gsp_matmul_batch: products of more than 64 rows may
  * need a workspace, so run the product, or a larger one, once before capturing

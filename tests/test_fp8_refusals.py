@@ -79,6 +79,7 @@ def test_matmul_refuses(kw):
 @pytest.mark.parametrize("kw", [
     dict(w_type=gp.WTYPE_F32), dict(w_type=gp.WTYPE_Q8_0), dict(w_type=gp.WTYPE_Q6_K), dict(w_type=99),
     dict(in_dim=0), dict(in_dim=32), dict(in_dim=480), dict(w_type=gp.WTYPE_Q4_K, in_dim=320),
+    dict(out_dim=(1 << 24) + 1), dict(out_dim=(1 << 31) - 1, batch=(1 << 31) - 1),
 ], ids=str)
 def test_matmul_unsupported(kw):
     assert matmul(**kw) == UNSUPPORTED and gp.load().gsp_last_error()

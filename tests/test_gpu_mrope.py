@@ -120,6 +120,33 @@ def test_matches_64_bits(torch_mod, gsp, ctx, case, layout, style, fused):
     pool.destroy()
 
 
+@pytest.mark.parametrize("case", [CASES[0], CASES[1], CASES[4]], ids=["d128", "d64", "odd"])
+def test_many_tokens(torch_mod, gsp, ctx, case):
+    """A prefill of over 512 tokens, whose threads take several items each."""
+    torch = torch_mod
+    heads, kvh, d, dv, rope_dim, sections, kv, page = case
+    rng = np.random.default_rng(31)
+    pool, blocks, blk, slot = _step(gsp, ctx, rng, case, n_rows=30, new_hi=50)
+    n = len(blk)
+    assert n >= 512
+    axes = rng.integers(0, 60000, (len(sections), n)).astype(np.int32)
+    q, k, v = (rng.standard_normal((n, w)).astype(np.float32) for w in (heads * d, kvh * d, kvh * dv))
+    qd, kd, vd, pos = (torch.from_numpy(t).cuda() for t in (q, k, v, axes))
+    torch.cuda.synchronize()
+    pool.mrope_write_step(0, heads, gsp.MRope(BASE, sections, 1, rope_dim=rope_dim), pos.data_ptr(), qd.data_ptr(),
+                          qd.data_ptr(), kd.data_ptr(), vd.data_ptr())
+    ctx.sync()
+    K, V = _arenas(pool, blocks, 2, case)
+    rates = BASE ** (-2.0 * np.arange(rope_dim // 2) / rope_dim)
+    axis = axis_of_pair(sections, False)
+    wantq, magq = rotate64(q.reshape(n, heads, d), axes, axis, rates, rope_dim, True)
+    wantk, magk = rotate64(k.reshape(n, kvh, d), axes, axis, rates, rope_dim, True)
+    assert np.all(np.abs(qd.cpu().numpy().reshape(wantq.shape) - wantq) <= _tol(magq, wantq, "f32"))
+    assert np.all(np.abs(K[blk, 0, :, slot].astype(np.float64) - wantk) <= _tol(magk, wantk, kv))
+    assert np.array_equal(V[blk, 0, :, slot], v.reshape(n, kvh, dv).astype(V.dtype))
+    pool.destroy()
+
+
 @pytest.mark.parametrize("tables", ["inv_freq", "factors"])
 def test_equal_axes_are_plain_rope(torch_mod, gsp, ctx, tables):
     """Text: the same position on every axis, at the token's place in its row, is gsp_rope_write_step_ex.
