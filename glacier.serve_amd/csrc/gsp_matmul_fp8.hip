@@ -751,6 +751,11 @@ __global__ __launch_bounds__(256) void add_splits_kernel(const float* part, floa
     }
 }
 
+// Converted activations of 16 rows take 8 KB a unit and 512 bytes of sums.  A call keeps at most 1 GB of them: more rows
+// are multiplied piece by piece, each of many more workgroups than the chip holds.
+constexpr int64_t kConverted = 8192 + 512;
+int64_t converted_rows(int units) { return std::max<int64_t>(1, (1 << 30) / (units * kConverted) / 8) * 128; }
+
 template <int WT, int MT, int NT, int WN, int G, bool PRE>
 hipError_t launch_tile(MatmulFp8Args a, int splits, hipStream_t stream) {
     const bool aligned = a.in_dim % 256 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
@@ -759,7 +764,8 @@ hipError_t launch_tile(MatmulFp8Args a, int splits, hipStream_t stream) {
     if (splits == 1) a.partials = nullptr;
     const int64_t tiles_n = ((int64_t)a.out_dim + 16 * NT * WN - 1) / (16 * NT * WN);
     // A launch holds fewer than 2^32 threads: very large batches take several (and no splits).
-    const int64_t most_rows = std::max<int64_t>(1, (1 << 21) / std::max<int64_t>(tiles_n, PRE ? units : 1)) * (16 * MT);
+    int64_t most_rows = std::max<int64_t>(1, (1 << 21) / std::max<int64_t>(tiles_n, PRE ? units : 1)) * (16 * MT);
+    if (PRE) most_rows = std::min(most_rows, converted_rows(units));
     for (int64_t left = a.batch; left > 0; left -= most_rows) {
         a.batch = (int32_t)std::min(left, most_rows);
         if constexpr (PRE) {
@@ -835,6 +841,7 @@ MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, in
     const int units = (in_dim + 255) / 256;
     double least = 0;
     for (const Form& f : kForms) {
+        if (batch <= f.rows / 2) continue;  // half of it empty: the next one takes less, and no workspace up to 64 rows
         const double tiles = (double)(((int64_t)batch + f.rows - 1) / f.rows) * (((int64_t)out_dim + f.cols - 1) / f.cols);
         int fit = 4;
         while (fit > 1 && f.us[fit - 1] == 0) --fit;
@@ -859,8 +866,9 @@ MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, in
 }
 
 int64_t matmul_fp8_x_bytes(int32_t in_dim, int32_t batch, const MatmulFp8Plan& plan) {
-    // 16 rows of a unit: 8 KB of activations, 512 bytes of sums.
-    return plan.form == MatmulFp8Plan::kTile128 ? ((int64_t)batch + 127) / 128 * 8 * ((in_dim + 255) / 256) * (8192 + 512) : 0;
+    if (plan.form != MatmulFp8Plan::kTile128) return 0;
+    const int units = (in_dim + 255) / 256;
+    return (std::min<int64_t>(batch, converted_rows(units)) + 127) / 128 * 8 * units * kConverted;
 }
 
 int64_t matmul_fp8_row_bytes(int32_t w_type, int32_t in_dim) {

@@ -322,7 +322,7 @@ int gsp_quantize_fp8(gsp_ctx* ctx, int32_t act, int32_t rows, int32_t dim, int64
  * need a workspace, so run the product, or a larger one, once before capturing
  * it (GSP_E_STATE otherwise, and nothing is enqueued); captured products keep
  * buffers of their own and their graphs must not run at the same time as each
- * other.  Up to 64 rows nothing is needed. */
+ * other.  Up to 64 rows nothing is needed; above, at most about 1 GB. */
 #define GSP_WTYPE_Q4_0 2
 #define GSP_WTYPE_Q4_1 3
 int gsp_matmul_batch_fp8(gsp_ctx* ctx, int32_t w_type, const void* w_dev, const uint8_t* x_dev,

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from fp8_helpers import E4M3, Q4_0, check_codes, decode_weights, norm64, random_weights
+from fp8_helpers import E4M3, Q4_0, Q4_1, check_codes, decode_weights, norm64, random_weights
 
 pytestmark = pytest.mark.gpu
 
@@ -86,4 +86,26 @@ def test_outputs_past_8_gb(torch_mod, gsp, ctx, in_dim):
     assert np.all(np.abs(y[-130:].cpu().numpy() - X @ wm.T) <= bound)
     assert not any(part.any() for part in y[:-130].split(8192))
     del y
+    _free(torch)
+
+
+def test_rows_in_pieces(torch_mod, gsp, ctx):
+    """More converted activations than the workspace holds at once: 3840 rows a piece at 512 units of K."""
+    torch = torch_mod
+    rng = np.random.default_rng(4)
+    in_dim, out_dim, batch = 131072, 520, 9001
+    raw = random_weights(rng, Q4_1, out_dim, in_dim)
+    x = torch.randint(0, 120, (batch, in_dim), dtype=torch.uint8, device="cuda")
+    w, s = torch.from_numpy(raw).cuda(), torch.ones(batch, device="cuda")
+    y = torch.zeros((batch, out_dim), device="cuda")
+    torch.cuda.synchronize()
+    ctx.matmul_batch_fp8(Q4_1, w.data_ptr(), x.data_ptr(), s.data_ptr(), y.data_ptr(), in_dim, out_dim, batch)
+    ctx.sync()
+    rows = [0, 1, 3711, 3839, 3840, 3841, 3967, 7679, 7680, 7681, 8999, 9000]
+    wm, mag = decode_weights(Q4_1, raw, in_dim)
+    X = E4M3[x[rows].cpu().numpy()]
+    bound = (37 + in_dim / 16) * 2.0 ** -23 * (np.abs(X) @ mag.T)
+    assert np.all(np.abs(y[rows].cpu().numpy() - X @ wm.T) <= bound)
+    assert not (y == 0).all(dim=1).any()
+    del x, y
     _free(torch)

@@ -300,3 +300,34 @@ def test_nan_rows_in_the_128_row_form(torch_mod, gsp, ctx):
     bad = torch.isnan(y).any(1).cpu().numpy()
     assert set(np.nonzero(bad)[0]) == {3, 200}
     assert torch.isnan(y[[3, 200]]).all()
+
+
+@pytest.mark.parametrize("out_dim", [130, 16400, 70000])
+@pytest.mark.parametrize("batch", [1, 33, 64])
+def test_cold_capture_up_to_64_rows(torch_mod, gsp, batch, out_dim):
+    """Products of up to 64 rows need no workspace: a context's first call may be captured."""
+    torch = torch_mod
+    ctx = gsp.Context(0)
+    stream = torch.cuda.Stream()
+    ctx.set_stream(stream.cuda_stream)
+    rng = np.random.default_rng(batch)
+    in_dim = 320
+    raw = random_weights(rng, Q4_1, out_dim, in_dim)
+    codes = rng.integers(0, 120, (batch, in_dim)).astype(np.uint8)
+    w, x = torch.from_numpy(raw).cuda(), torch.from_numpy(codes).cuda()
+    s, y = torch.ones(batch, device="cuda"), torch.zeros((batch, out_dim), device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        ctx.matmul_batch_fp8(Q4_1, w.data_ptr(), x.data_ptr(), s.data_ptr(), y.data_ptr(), in_dim, out_dim, batch)
+    wm, mag = decode_weights(Q4_1, raw, in_dim)
+    X = E4M3[codes]
+    bound = (37 + in_dim / 16) * 2.0 ** -23 * (np.abs(X) @ mag.T)
+    for _ in range(2):
+        y.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert np.all(np.abs(y.cpu().numpy() - X @ wm.T) <= bound)
+    del g
+    ctx.close()
