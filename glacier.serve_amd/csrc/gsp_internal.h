@@ -237,7 +237,7 @@ struct MatmulFp8Args {
 };
 // The kernel that a product takes, and the ranges of K that share an output (several only with a tile form).
 struct MatmulFp8Plan {
-    enum { kStream = 0, kTile128, kTile64, kTile32 };
+    enum { kStream = 0, kWide, kTile64, kTile32 };
     int32_t form = kStream;
     int32_t splits = 1;
     int32_t cus = 1;

@@ -33,6 +33,7 @@ namespace gsp {
 namespace {
 
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
@@ -408,6 +409,7 @@ hipError_t launch_form(MatmulFp8Args a, hipStream_t stream) {
 
 // Keeps a value's computation from being moved behind this point, or folded into its uses.
 __device__ inline void pin(f4& v) { asm volatile("" : "+v"(v)); }
+__device__ inline void pin(f16v& v) { asm volatile("" : "+v"(v)); }
 __device__ inline void pin(float& v) { asm volatile("" : "+v"(v)); }
 
 // LDS traffic of the wave is done; the other waves' too after the barrier.
@@ -419,90 +421,66 @@ __device__ inline void lds_barrier() {
 }
 
 // The tile form, for batches that use an expanded weight many times: 16 * MT
-// batch rows by 16 * NT * WN weight rows a workgroup.  Activations lie in LDS as
-// fp16, in the order the instruction's operands take, 32 G of K at a time in two
-// buffers: each workgroup converts its own (PRE false), or they come converted from
-// matmul_fp8_convert_kernel (PRE), which pays for its launch where many workgroups
-// share rows (3584 x 18944 at 2048 rows: 361 -> 345 us).  Each wave has its own
-// weight rows, in a slot as above.
+// batch rows by 16 * WN weight rows a workgroup.  Each converts its activations to
+// fp16 in LDS, in the order the instruction's operands take, 128 of K at a time in
+// two buffers.  Each wave has its own 16 weight rows, in a slot as above.
 //
 // The matrix and the vector units work beside each other: while the products of one
-// set (16 weight rows, all batch rows, one group) run, the previous set's sums are
-// scaled into the outputs' (Q4_0 and Q4_1: one fused multiply-add an output and group
-// is the vector unit's main work) and the next set's weights are expanded.  Q4_K's
-// scales are integers within the operand, so that its sums run over the eight groups
-// of a super-block in the matrix unit alone.  Minimums meet the sums of x in one more
-// product a unit: staging adds up each group, and leaves its sum as two fp16 numbers,
-// the nearest and what that leaves (22 bits; a sum has up to 23).
-template <int WT, int MT, int NT, int WN, int G, bool PRE, bool AL>
+// group run, the previous group's sums are scaled into the outputs' (Q4_0 and Q4_1: one
+// fused multiply-add an output and group is the vector unit's main work) and the next
+// group's weights are expanded.  Q4_K's scales are integers within the operand, so that
+// its sums run over the eight groups of a super-block in the matrix unit alone.
+// Minimums meet the sums of x in one more product a unit: staging adds up each group,
+// and leaves its sum as two fp16 numbers, the nearest and what that leaves (22 bits; a
+// sum has up to 23).
+//
+// Two heights: 64 rows by 128 (Q4_0, 3584 x 3584 at 512 rows 31.6 us, 416 TFLOP/s) and
+// 32 by 64 where that fills the chip better (896 x 4864 at 65 rows 7.8 us).
+template <int WT, int MT, int WN, bool AL>
 __global__ __launch_bounds__(64 * WN) void matmul_fp8_tile_kernel(MatmulFp8Args a) {
     constexpr int kRow = Unit<WT>::kRow, kTile = 16 * kRow;
-    constexpr int kSteps = 8 / G;                            // of a unit, G groups of 32 each
+    constexpr int G = 4, kSteps = 8 / G;                       // steps of a unit, G groups of 32 each
     constexpr int kStep = MT * G * 1024;                     // LDS bytes of a step's activations
     constexpr int kRowPieces = 2 * G;                        // 16-byte pieces of a row in a step
     constexpr int kPieces = MT * 16 * kRowPieces / (64 * WN);  // pieces a thread stages
-    constexpr int kBlocks = MT * G / WN;                       // KB that a wave loads of a converted step
-    static_assert(kPieces * 64 * WN == MT * 16 * kRowPieces && (!PRE || (kBlocks * WN == MT * G && MT == WN)), "even shares");
-    static_assert(!PRE || kSteps == 2, "the waits count a unit of two steps");
-    // Two arrays, so that the compiler sees that loads into one do not concern reads of the other.
+    static_assert(kPieces * 64 * WN == MT * 16 * kRowPieces, "even shares");
     __shared__ __attribute__((aligned(16))) uint8_t xs0[kStep];
     __shared__ __attribute__((aligned(16))) uint8_t xs1[kStep];
     const auto x_buf = [&](int step) { return step % 2 ? xs1 : xs0; };
-    __shared__ __attribute__((aligned(16))) uint8_t ws[WN][NT * kTile];
+    __shared__ __attribute__((aligned(16))) uint8_t ws[WN][kTile];
     constexpr bool kMins = Unit<WT>::kMins;
     __shared__ __attribute__((aligned(16))) _Float16 gs[kMins ? 2 : 1][kMins ? MT : 1][2][16][8];  // group sums of two units
     __shared__ __attribute__((aligned(16))) float scales[16 * MT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, j = lane >> 4;
-    const int tiles_b = (a.batch + 16 * MT - 1) / (16 * MT), tiles_n = (a.out_dim + 16 * NT * WN - 1) / (16 * NT * WN);
+    const int tiles_b = (a.batch + 16 * MT - 1) / (16 * MT), tiles_n = (a.out_dim + 16 * WN - 1) / (16 * WN);
     // Workgroups go to the eight XCDs in turn: each XCD gets a run of tiles that share weight rows.
     const int tiles = tiles_b * tiles_n;
     const int split = blockIdx.x / tiles;
     int tile = blockIdx.x % tiles;
     const int per_xcd = tiles / 8;
     if (tile < per_xcd * 8) tile = tile % 8 * per_xcd + tile / 8;
-    const int row0 = (tile / tiles_b * WN + wave) * (16 * NT), b0 = tile % tiles_b * (16 * MT);
+    const int row0 = (tile / tiles_b * WN + wave) * 16, b0 = tile % tiles_b * (16 * MT);
     // This split's units of K.
     const int pairs = a.in_dim >> 6;
     const int units = (pairs + 3) >> 2, u0 = split * a.units_per_split, u1 = min(u0 + a.units_per_split, units);
 
     // Weights: 16 rows' offsets fit 32 bits.  Rows behind the last are the last again.
     const auto send = [&](int u) {
+        const int first = min(row0, a.out_dim - 1), rows = a.out_dim - 1 - first;
+        const uint8_t* base = static_cast<const uint8_t*>(a.w) + (int64_t)first * a.row_bytes + (int64_t)u * kRow;
+        const uint32_t left = (uint32_t)(a.row_bytes - (int64_t)u * kRow - 4);
+        const auto at_byte = [&](int byte) {
+            const int r = byte / kRow;
+            uint32_t col = byte % kRow;
+            if constexpr (!AL) col = min(col, left);
+            return base + (uint64_t)((uint32_t)min(r, rows) * (uint32_t)a.row_bytes + col);
+        };
+        constexpr int kWide = AL ? kTile / 1024 * 1024 : 0;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const int first = min(row0 + 16 * i, a.out_dim - 1), rows = a.out_dim - 1 - first;
-            const uint8_t* base = static_cast<const uint8_t*>(a.w) + (int64_t)first * a.row_bytes + (int64_t)u * kRow;
-            const uint32_t left = (uint32_t)(a.row_bytes - (int64_t)u * kRow - 4);
-            const auto at_byte = [&](int byte) {
-                const int r = byte / kRow;
-                uint32_t col = byte % kRow;
-                if constexpr (!AL) col = min(col, left);
-                return base + (uint64_t)((uint32_t)min(r, rows) * (uint32_t)a.row_bytes + col);
-            };
-            uint8_t* to = &ws[wave][i * kTile];
-            constexpr int kWide = AL ? kTile / 1024 * 1024 : 0;
+        for (int at = 0; at < kWide; at += 1024) load_to_lds<16>(at_byte(at + 16 * lane), ws[wave] + at);
 #pragma unroll
-            for (int at = 0; at < kWide; at += 1024) load_to_lds<16>(at_byte(at + 16 * lane), to + at);
-#pragma unroll
-            for (int at = kWide; at < kTile; at += 256) load_to_lds<4>(at_byte(at + 4 * lane), to + at);
-        }
-    };
-    // Loads of a unit's weights, which the wait below counts.
-    constexpr int kWide16 = AL ? kTile / 1024 : 0;
-    constexpr int kSent = NT * (kWide16 + (kTile - 1024 * kWide16) / 256);
-    // Converted activations (PRE): a step's KB of 16 rows and a group each, and a unit's group sums, a tile a wave.
-    const auto send_x = [&](int step, uint8_t* to) {
-#pragma unroll
-        for (int i = 0; i < kBlocks; ++i) {
-            const int kb = wave * kBlocks + i, m = kb / G, g = kb % G;
-            const int64_t at = ((int64_t)(b0 / 16 + m) * units * 8 + step * G + g) * 1024;
-            load_to_lds<16>(a.xf + at + 16 * lane, to + kb * 1024);
-        }
-    };
-    const auto send_sums = [&](int u) {
-        if (lane < 32)
-            load_to_lds<16>(a.sums + ((int64_t)(b0 / 16 + wave) * units + u) * 512 + 16 * lane,
-                            reinterpret_cast<uint8_t*>(&gs[u % 2][kMins ? wave : 0][0][0][0]));
+        for (int at = kWide; at < kTile; at += 256) load_to_lds<4>(at_byte(at + 4 * lane), ws[wave] + at);
     };
     // Piece i of a thread: 16 bytes of a row, neighbouring lanes on neighbouring pieces.
     u4 piece[kPieces];
@@ -542,53 +520,31 @@ __global__ __launch_bounds__(64 * WN) void matmul_fp8_tile_kernel(MatmulFp8Args 
             }
         }
     };
-    // The operand of one group and of the next.  Q4_K, whose super-block's sums take those registers, reads the next one
-    // in place behind the last product that uses it: 364 us for 2048 rows of 3584 by 18944, two operands (spilled) 396.
-    constexpr bool kWholeBlock = WT == GSP_WTYPE_Q4_K;
-    constexpr int kAhead = kWholeBlock ? 1 : 2;
-    Terms xt[kAhead][MT];
-    const int read_at[2] = {lane * 16, (PRE ? lane : lane ^ 8) * 16};
-    const auto read_tile = [&](const uint8_t* buf, int g, int m) {
-        xt[g % kAhead][m] =
-            __builtin_bit_cast(Terms, *reinterpret_cast<const u4*>(buf + (m * G + g) * 1024 + read_at[g % 2]));
-    };
+    // The operands of one group and of the next.
+    Terms xt[2][MT];
+    const int read_at[2] = {lane * 16, (lane ^ 8) * 16};
     const auto read_x = [&](const uint8_t* buf, int g) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) read_tile(buf, g, m);
+        for (int m = 0; m < MT; ++m)
+            xt[g % 2][m] =
+                __builtin_bit_cast(Terms, *reinterpret_cast<const u4*>(buf + (m * G + g) * 1024 + read_at[g % 2]));
     };
 
-    constexpr int kSets = G * NT;  // of a step, in the order group, 16 weight rows
-    f4 acc[NT][MT];
+    constexpr bool kWholeBlock = WT == GSP_WTYPE_Q4_K;
+    f4 acc[MT];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m) acc[i][m] = f4{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int m = 0; m < MT; ++m) acc[m] = f4{0.f, 0.f, 0.f, 0.f};
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
     uint32_t mask = kNib;
     asm volatile("" : "+v"(mask));
-    f4 sum[kWholeBlock ? NT : 2][MT];  // Q4_K: the super-block's sums; else the last two sets'
+    f4 sum[kWholeBlock ? 1 : 2][MT];  // Q4_K: the super-block's sums; else the last two groups'
     const uint32_t keep = j < 2 ? 0xffffffffu : 0u;
-    Dealt<WT> w[NT];
-    const auto take_w = [&](int u) {  // unit u has landed; the next one is sent for
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        Unit<WT> raw[NT];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) raw[i].read(&ws[wave][i * kTile], n, j);
-#pragma unroll
-        for (int i = 0; i < NT; ++i) w[i].deal(raw[i]);
-    };
+    Dealt<WT> w;
     send(u0);
     if (threadIdx.x < 16 * MT) scales[threadIdx.x] = a.x_scale[min(b0 + (int)threadIdx.x, a.batch - 1)];
-    if constexpr (PRE) {
-        if constexpr (kMins) send_sums(u0);
-        send_x(kSteps * u0, x_buf(0));
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    } else {
-        fetch_x(kSteps * u0);
-        stage_x(kSteps * u0, x_buf(0));
-        fetch_x(kSteps * u0 + 1);
-    }
+    fetch_x(kSteps * u0);
+    stage_x(kSteps * u0, x_buf(0));
+    fetch_x(kSteps * u0 + 1);
     lds_barrier();
     read_x(x_buf(0), 0);
     float sc_last = 0.f;
@@ -597,88 +553,61 @@ __global__ __launch_bounds__(64 * WN) void matmul_fp8_tile_kernel(MatmulFp8Args 
         for (int m = 0; m < MT; ++m) sum[1][m] = zero;
     }
     for (int u = u0; u < u1; ++u) {
-        take_w(u);
-        Terms q = w[0].operand(0, 0, mask);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the unit's weights have landed
+        Unit<WT> raw;
+        raw.read(ws[wave], n, j);
+        w.deal(raw);
+        Terms q = w.operand(0, 0, mask);
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             // The buffer written here was last read before the barrier below, in the step before.  At the end the last
-            // step and unit are loaded again, for nobody, so that the waits' counts hold.
-            const int last_step = kSteps * u1 - 1;
-            if constexpr (PRE) {
-                send_x(min(kSteps * u + s + 1, last_step), x_buf(s + 1));
-            } else {
-                stage_x(kSteps * u + s + 1, x_buf(s + 1));
-                fetch_x(min(kSteps * u + s + 2, last_step));
-            }
+            // step and unit are loaded again, for nobody.
+            stage_x(kSteps * u + s + 1, x_buf(s + 1));
+            fetch_x(min(kSteps * u + s + 2, kSteps * u1 - 1));
             if (s == 0) {
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the unit's weights are in registers
                 send(min(u + 1, u1 - 1));
             }
 #pragma unroll
-            for (int k = 0; k < kSets; ++k) {
-                const int g = k / NT, i = k % NT, ug = s * G + g, t = ug / 2, h = ug % 2;
-                const int last_i = (k + kSets - 1) % kSets % NT;
-                if (g == G - 1 && i == 0) {
-                    // The next step's activations are staged, this step's in registers.  PRE: loads complete in order, and
-                    // behind the next step's only the next unit's weights were sent for, in a unit's first step.
-                    if constexpr (PRE) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(s == 0 ? kSent : 0) : "memory");
-                    lds_barrier();
-                    if constexpr (PRE && kMins)
-                        if (s == 0) send_sums(min(u + 1, u1 - 1));  // every wave is past the sums of the unit before
-                }
-                const uint8_t* next_x = x_buf(g < G - 1 ? s : s + 1);
-                if (kAhead == 2 && i == 0) read_x(next_x, (g + 1) % G);
-                const bool live = AL || 4 * u + t < pairs;
+            for (int g = 0; g < G; ++g) {
+                const int ug = s * G + g, t = ug / 2, h = ug % 2;
+                if (g == G - 1) lds_barrier();  // the next step's activations are staged, this step's in registers
+                read_x(x_buf(g < G - 1 ? s : s + 1), (g + 1) % G);
                 float sc = 0.f;
-                if constexpr (!kWholeBlock) sc = live ? w[i].scale(t, h) : 0.f;
+                if constexpr (!kWholeBlock) sc = AL || 4 * u + t < pairs ? w.scale(t, h) : 0.f;
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                     if constexpr (kWholeBlock) {
-                        sum[i][m] = mfma(xt[0][m], q, ug == 0 ? zero : sum[i][m]);
-                        if (i == NT - 1) read_tile(next_x, (g + 1) % G, m);
+                        sum[0][m] = mfma(xt[g % 2][m], q, ug == 0 ? zero : sum[0][m]);
                     } else {
-                        sum[k % 2][m] = mfma(xt[g % 2][m], q, zero);
-                    }
-                    if constexpr (!kWholeBlock) {
+                        sum[g % 2][m] = mfma(xt[g % 2][m], q, zero);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[last_i][m][r] = fmaf(sc_last, sum[(k + 1) % 2][m][r], acc[last_i][m][r]);
+                        for (int r = 0; r < 4; ++r) acc[m][r] = fmaf(sc_last, sum[(g + 1) % 2][m][r], acc[m][r]);
                     }
                 }
-                if (k + 1 < kSets || s + 1 < kSteps) {
-                    const int k2 = (k + 1) % kSets, g2 = (s + (k + 1) / kSets) * G + k2 / NT;
-                    q = w[k2 % NT].operand(g2 / 2, g2 % 2, mask);
-                }
+                if (ug < 7) q = w.operand((ug + 1) / 2, (ug + 1) % 2, mask);
                 sc_last = sc;
                 pin(sc_last);
 #pragma unroll
-                for (int m = 0; m < MT; ++m) pin(acc[last_i][m]);
+                for (int m = 0; m < MT; ++m) pin(acc[m]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
         if constexpr (kMins) {
-            Terms ms[MT], mn[NT];
+            Terms mn = w.minimums(keep);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) ms[m] = __builtin_bit_cast(Terms, *reinterpret_cast<const u4*>(&gs[u % 2][m][j & 1][n][0]));
+            for (int t = 0; t < 4; ++t)
+                if (!AL && 4 * u + t >= pairs) mn.r[t] = 0;
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                mn[i] = w[i].minimums(keep);
+            for (int m = 0; m < MT; ++m) {
+                const Terms ms = __builtin_bit_cast(Terms, *reinterpret_cast<const u4*>(&gs[u % 2][m][j & 1][n][0]));
+                if constexpr (kWholeBlock) {
+                    const f4 low = mfma(ms, mn, zero);
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    if (!AL && 4 * u + t >= pairs) mn[i].r[t] = 0;
-            }
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    if constexpr (kWholeBlock) {
-                        const f4 low = mfma(ms[m], mn[i], zero);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            acc[i][m][r] = fmaf(w[i].d, sum[i][m][r], fmaf(-w[i].dmin, low[r], acc[i][m][r]));
-                        pin(acc[i][m]);
-                    } else {
-                        acc[i][m] = mfma(ms[m], mn[i], acc[i][m]);
-                    }
+                    for (int r = 0; r < 4; ++r) acc[m][r] = fmaf(w.d, sum[0][m][r], fmaf(-w.dmin, low[r], acc[m][r]));
+                    pin(acc[m]);
+                } else {
+                    acc[m] = mfma(ms, mn, acc[m]);
                 }
             }
         }
@@ -687,37 +616,360 @@ __global__ __launch_bounds__(64 * WN) void matmul_fp8_tile_kernel(MatmulFp8Args 
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[NT - 1][m][r] = fmaf(sc_last, sum[1][m][r], acc[NT - 1][m][r]);
+            for (int r = 0; r < 4; ++r) acc[m][r] = fmaf(sc_last, sum[1][m][r], acc[m][r]);
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load outlives the loop
     float* y = a.partials ? a.partials + (int64_t)split * a.batch * a.out_dim : a.y;
-    const bool whole = b0 + 16 * MT <= a.batch && row0 + 16 * NT <= a.out_dim;
+    const bool whole = b0 + 16 * MT <= a.batch && row0 + 16 <= a.out_dim;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         const f4 f = *reinterpret_cast<const f4*>(&scales[16 * m + 4 * j]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int b = b0 + 16 * m + 4 * j + r;
-            float* to = y + (int64_t)b * a.out_dim + row0 + n;
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-                if (whole || (b < a.batch && row0 + 16 * i + n < a.out_dim)) to[16 * i] = acc[i][m][r] * f[r];
+            if (whole || (b < a.batch && row0 + n < a.out_dim)) y[(int64_t)b * a.out_dim + row0 + n] = acc[m][r] * f[r];
         }
     }
 }
 
-// Activations for the tile form whose workgroups are many enough that converting
-// them once before pays for a launch: fp16 in the operand's order, [16 rows][group]
-// of 1 KB, lane (row, j)'s 16 bytes behind each other, and each group's sum as two
-// fp16 numbers, [16 rows][unit][2][row][group].  Rows and groups past the end are 0.
-// A thread converts one group of a row.
-__global__ __launch_bounds__(128) void matmul_fp8_convert_kernel(const uint8_t* x, uint8_t* xf, _Float16* sums, int in_dim,
+// 256 weights of each of 32 rows for the wide tile form's instructions (32 x 32 x 16, two
+// a group of 32 weights: lane (n, h) = (lane % 32, lane / 32) holds dwords 2h + p of
+// row n in the p-th).  A lane reads half a row's blocks from LDS and trades every
+// second register with the lane of the other half.
+template <int WT>
+struct Rows {
+    uint32_t q[16];  // bytes in the order 0 2 1 3; Q4_0, Q4_1: group g's p-th at 2 g + p; Q4_K: a pair of groups' at 4, + 2 p
+    uint32_t s[8];   // Q4_0: two groups' d each; Q4_1: a group's d and m; Q4_K: four scales, four, four minimums, four
+    float d, dmin;   // Q4_K: of the super-block
+
+    __device__ inline void read(const uint8_t* rows, int n, int h) {
+        const uint8_t* p = rows + n * Unit<WT>::kRow;
+        if constexpr (WT == GSP_WTYPE_Q4_K) {
+            const u4 head = *reinterpret_cast<const u4*>(p);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const u4 a = *reinterpret_cast<const u4*>(p + 16 + 64 * h + 32 * c);
+                const u4 b = *reinterpret_cast<const u4*>(p + 32 + 64 * h + 32 * c);
+                // Dword i of a byte row belongs to lane half i / 2.
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t a0 = deal_bytes(a[i]), a1 = deal_bytes(a[2 + i]), b0 = deal_bytes(b[i]), b1 = deal_bytes(b[2 + i]);
+                    swap32(a0, a1);
+                    swap32(b0, b1);
+                    q[4 * c + 2 * i] = a0, q[4 * c + 2 * i + 1] = b0;
+                    q[8 + 4 * c + 2 * i] = a1, q[8 + 4 * c + 2 * i + 1] = b1;
+                }
+            }
+            d = half_lo(head[0]);
+            dmin = half_hi(head[0]);
+            s[0] = head[1] & 0x3f3f3f3fu;
+            s[1] = (head[3] & 0x0f0f0f0fu) | (head[1] & 0xc0c0c0c0u) >> 2;
+            s[2] = head[2] & 0x3f3f3f3fu;
+            s[3] = (head[3] >> 4 & 0x0f0f0f0fu) | (head[2] & 0xc0c0c0c0u) >> 2;
+        } else {
+            constexpr int kWords = Unit<WT>::kRow / 8;
+            uint32_t w[kWords];
+#pragma unroll
+            for (int i = 0; i < kWords; i += 2) {
+                const u2 two = *reinterpret_cast<const u2*>(p + 4 * kWords * h + 4 * i);
+                w[i] = two[0], w[i + 1] = two[1];
+            }
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                uint32_t e[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (WT == GSP_WTYPE_Q4_1)
+                        e[i] = deal_bytes(w[5 * b + 1 + i]);
+                    else if (b % 2)
+                        e[i] = deal_bytes(w[9 * (b / 2) + 5 + i]);
+                    else  // between two dwords
+                        e[i] = __builtin_amdgcn_perm(w[9 * (b / 2) + i + 1], w[9 * (b / 2) + i], 0x05030402u);
+                }
+                swap32(e[0], e[2]);
+                swap32(e[1], e[3]);
+                q[2 * b] = e[0], q[2 * b + 1] = e[1], q[8 + 2 * b] = e[2], q[8 + 2 * b + 1] = e[3];
+            }
+            constexpr int kScales = WT == GSP_WTYPE_Q4_1 ? 4 : 2;  // dwords a lane
+#pragma unroll
+            for (int i = 0; i < kScales; ++i) {
+                uint32_t a = WT == GSP_WTYPE_Q4_1 ? w[5 * i] : (w[9 * i] & 0xffffu) | (w[9 * i + 4] & 0xffff0000u), b = a;
+                swap32(a, b);
+                s[i] = a, s[kScales + i] = b;
+            }
+        }
+    }
+    // The p-th operand of group g: q - 8 (Q4_0) and q times the group's 6-bit scale, an exact integer up to 945 (Q4_K),
+    // formed from 1024 + 16 q in one fused step, or q times 1 / kCode (Q4_1).  mask: kNib in a register.
+    __device__ inline Terms operand(int g, int p, uint32_t mask) const {
+        if constexpr (WT == GSP_WTYPE_Q4_1) {
+            const uint32_t a = q[2 * g + p];
+            return Terms{{(a << 4) & mask, (a >> 4) & mask, a & mask, (a >> 8) & mask}};
+        }
+        h2 f = {0.0625f16, 0.0625f16}, c = {-72.f16, -72.f16};
+        if constexpr (WT == GSP_WTYPE_Q4_K) {
+            const float sc = (float)((s[g / 4] >> (8 * (g % 4))) & 0xffu) * 0.0625f;
+            f = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(sc, sc));
+            c = f * h2{-1024.f16, -1024.f16};
+        }
+        const auto make = [&](uint32_t w) {
+            return __builtin_bit_cast(
+                uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & mask) | 0x64006400u), f, c));
+        };
+        const uint32_t a = WT == GSP_WTYPE_Q4_K ? q[g / 2 * 4 + 2 * p] : q[2 * g + p];
+        const uint32_t b = WT == GSP_WTYPE_Q4_K ? q[g / 2 * 4 + 2 * p + 1] : a;
+        if (WT == GSP_WTYPE_Q4_K && g % 2) return Terms{{make(a), make(a >> 8), make(b), make(b >> 8)}};
+        if (WT == GSP_WTYPE_Q4_K) return Terms{{make(a << 4), make(a >> 4), make(b << 4), make(b >> 4)}};
+        return Terms{{make(a << 4), make(a >> 4), make(a), make(a >> 8)}};
+    }
+    // What a group's sum of products enters with.
+    __device__ inline float scale(int g) const {
+        if constexpr (WT == GSP_WTYPE_Q4_1) return half_lo(s[g]) * kCode;
+        return g % 2 ? half_hi(s[g / 2]) : half_lo(s[g / 2]);
+    }
+    // What the eight groups' sums of x enter with, as fp16: m (Q4_1) or the 6-bit minimum (Q4_K).
+    __device__ inline Terms minimums() const {
+        Terms t;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (WT == GSP_WTYPE_Q4_K) {
+                const uint32_t two = s[2 + i / 2] >> (16 * (i % 2));
+                t.r[i] = __builtin_bit_cast(uint32_t,
+                                            __builtin_amdgcn_cvt_pkrtz((float)(two & 0xffu), (float)(two >> 8 & 0xffu)));
+            } else {
+                t.r[i] = __builtin_amdgcn_perm(s[2 * i + 1], s[2 * i], 0x07060302u);
+            }
+        }
+        return t;
+    }
+};
+
+__device__ inline f16v mfma32(const Terms& a, const Terms& b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+// The wide tile form: 128 batch rows by 256 weight rows a workgroup, 128 by 32 a wave,
+// in the 32 x 32 x 16 instruction, of which half as many are issued for the same terms.
+// Beside a multiply-add for each output it takes 9.3 ns a SIMD for 16 x 16 x 32 terms,
+// the other one 11.2, and issue is what bounds this form: the vector unit is busy 72 %
+// of the time (Q4_0, 18944 x 3584 at 2048 rows), with 512 multiply-adds, 176
+// instructions of expansion, 64 products and 63 others a wave and unit; the matrix unit
+// 45 %.  Activations come converted from matmul_fp8_convert_kernel, as converting them
+// in every workgroup took 4 % longer there.  us at 2048 rows (TFLOP/s), 3584 x 18944
+// and 18944 x 3584: Q4_0 332 (837) and 320, Q4_1 333 and 330, Q4_K 313 and 302.
+//
+// Measured without gain: the loads to LDS sent one by one between the products, the
+// weights read before their unit begins, activations through registers, the barrier
+// behind a product, and 32 x 32 x 16 tiles of 64 or 32 rows (3584 x 3584 at 512 rows
+// 40 us instead of 32: too few waves a SIMD).
+constexpr int kWideRows = 128, kWideWaves = 8;
+template <int WT, bool AL>
+__global__ __launch_bounds__(64 * kWideWaves) void matmul_fp8_wide_kernel(MatmulFp8Args a) {
+    constexpr int kRow = Unit<WT>::kRow, kTile = 16 * kRow;
+    constexpr int MT = kWideRows / 32, WN = kWideWaves, G = 4, kSteps = 8 / G;  // steps of a unit, G groups of 32 each
+    constexpr int kStep = MT * G * 2048;      // LDS bytes of a step's activations
+    constexpr int kBlocks = 2 * MT * G / WN;  // KB that a wave loads of them
+    static_assert(kBlocks * WN == 2 * MT * G && 2 * MT == WN, "even shares");
+    // Two arrays, so that the compiler sees that loads into one do not concern reads of the other.
+    __shared__ __attribute__((aligned(16))) uint8_t xs0[kStep];
+    __shared__ __attribute__((aligned(16))) uint8_t xs1[kStep];
+    const auto x_buf = [&](int step) { return step % 2 ? xs1 : xs0; };
+    __shared__ __attribute__((aligned(16))) uint8_t ws[WN][2 * kTile];
+    constexpr bool kMins = Unit<WT>::kMins;
+    __shared__ __attribute__((aligned(16))) _Float16 gs[kMins ? 2 : 1][kMins ? MT : 1][2][32][8];  // group sums of two units
+    __shared__ __attribute__((aligned(16))) float scales[32 * MT];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, h = lane >> 5;
+    const int tiles_b = (a.batch + 32 * MT - 1) / (32 * MT), tiles_n = (a.out_dim + 32 * WN - 1) / (32 * WN);
+    // Workgroups go to the eight XCDs in turn: each XCD gets a run of tiles that share weight rows.
+    const int tiles = tiles_b * tiles_n;
+    const int split = blockIdx.x / tiles;
+    int tile = blockIdx.x % tiles;
+    const int per_xcd = tiles / 8;
+    if (tile < per_xcd * 8) tile = tile % 8 * per_xcd + tile / 8;
+    const int row0 = (tile / tiles_b * WN + wave) * 32, b0 = tile % tiles_b * (32 * MT);
+    // This split's units of K.
+    const int pairs = a.in_dim >> 6;
+    const int units = (pairs + 3) >> 2, u0 = split * a.units_per_split, u1 = min(u0 + a.units_per_split, units);
+
+    // Weights: 16 rows' offsets fit 32 bits.  Rows behind the last are the last again.
+    constexpr int kWide16 = AL ? kTile / 1024 : 0, kTileLoads = kWide16 + (kTile - 1024 * kWide16) / 256;
+    constexpr int kLoads = 2 * kTileLoads;  // of a unit's weights
+    const auto send_w = [&](int u, int load) {
+        const int i = load / kTileLoads, k = load % kTileLoads;
+        const int first = min(row0 + 16 * i, a.out_dim - 1), rows = a.out_dim - 1 - first;
+        const uint8_t* base = static_cast<const uint8_t*>(a.w) + (int64_t)first * a.row_bytes + (int64_t)u * kRow;
+        const uint32_t left = (uint32_t)(a.row_bytes - (int64_t)u * kRow - 4);
+        const int at = k < kWide16 ? 1024 * k : 1024 * kWide16 + 256 * (k - kWide16);
+        const int byte = at + (k < kWide16 ? 16 : 4) * lane, r = byte / kRow;
+        uint32_t col = byte % kRow;
+        if constexpr (!AL) col = min(col, left);
+        const uint8_t* from = base + (uint64_t)((uint32_t)min(r, rows) * (uint32_t)a.row_bytes + col);
+        if (k < kWide16)
+            load_to_lds<16>(from, &ws[wave][i * kTile + at]);
+        else
+            load_to_lds<4>(from, &ws[wave][i * kTile + at]);
+    };
+    // Converted activations: a step's KB of half the operands of 32 rows and a group each, and a unit's group sums, half
+    // of 32 rows a wave.
+    const auto send_x = [&](int step, uint8_t* to, int load) {
+        const int kb = wave * kBlocks + load, m = kb / (2 * G), half = kb % (2 * G);
+        const int64_t at = (((int64_t)(b0 / 32 + m) * units * 8 + step * G) * 2 + half) * 1024;
+        load_to_lds<16>(a.xf + at + 16 * lane, to + kb * 1024);
+    };
+    const auto send_sums = [&](int u) {
+        if (lane < 32)
+            load_to_lds<16>(a.sums + (((int64_t)(b0 / 32 + wave / 2) * units + u) * 2 + wave % 2) * 512 + 16 * lane,
+                            reinterpret_cast<uint8_t*>(&gs[kMins ? u % 2 : 0][kMins ? wave / 2 : 0][wave % 2][0][0]));
+    };
+    // A group's operands, replaced in place by the next group's behind the products that use them.
+    Terms xt[MT][2];
+    const auto read_x = [&](const uint8_t* buf, int g, int m) {
+        const uint8_t* from = buf + (m * G + g) * 2048 + h * 512 + n * 16;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) xt[m][p] = __builtin_bit_cast(Terms, *reinterpret_cast<const u4*>(from + p * 1024));
+    };
+
+    constexpr bool kWholeBlock = WT == GSP_WTYPE_Q4_K;
+    // Sums of a super-block, or of the last products, all but one of them on the way (two instead of four: 2 % longer).
+    constexpr int kBuf = MT, kBehind = kBuf - 1;
+    const f16v zero = {};
+    f16v acc[MT], sum[kBuf];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m] = zero;
+    uint32_t mask = kNib;
+    asm volatile("" : "+v"(mask));
+    Rows<WT> w;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) send_w(u0, i);
+    if (threadIdx.x < 32 * MT) scales[threadIdx.x] = a.x_scale[min(b0 + (int)threadIdx.x, a.batch - 1)];
+    if constexpr (kMins) send_sums(u0);
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) send_x(kSteps * u0, x_buf(0), i);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
+#pragma unroll
+    for (int m = 0; m < MT; ++m) read_x(x_buf(0), 0, m);
+    float sc_last = 0.f;
+    if constexpr (!kWholeBlock) {
+#pragma unroll
+        for (int i = 0; i < kBuf; ++i) sum[i] = zero;
+    }
+    const auto add = [&](int m, float sc, const f16v& s, int from) {
+#pragma unroll
+        for (int r = from; r < from + 8; ++r) acc[m][r] = fmaf(sc, s[r], acc[m][r]);
+    };
+    for (int u = u0; u < u1; ++u) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the unit's weights have landed
+        w.read(ws[wave], n, h);
+        Terms q[2] = {w.operand(0, 0, mask), w.operand(0, 1, mask)};
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            // The buffer written in this step was last read before the barrier below, in the step before.  At the end the
+            // last step and unit are loaded again, for nobody, so that the waits' counts hold.
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i) send_x(min(kSteps * u + s + 1, kSteps * u1 - 1), x_buf(s + 1), i);
+            if (s == 0) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the unit's weights are in registers
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) send_w(min(u + 1, u1 - 1), i);
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int ug = s * G + g;
+                Terms next[2];
+                float sc = 0.f;
+                if constexpr (!kWholeBlock) sc = AL || 4 * u + ug / 2 < pairs ? w.scale(ug) : 0.f;
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    if (g == G - 1 && m == 0) {
+                        // The next step's activations have landed, this step's are in registers.  Loads complete in order,
+                        // and behind the next step's only the next unit's weights were sent for, in a unit's first step.
+                        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(s == 0 ? kLoads : 0) : "memory");
+                        lds_barrier();
+                        if constexpr (kMins)
+                            if (s == 0) send_sums(min(u + 1, u1 - 1));  // every wave is past the sums of the unit before
+                    }
+                    if constexpr (kWholeBlock) {
+                        sum[m] = mfma32(xt[m][0], q[0], ug == 0 ? zero : sum[m]);
+                        sum[m] = mfma32(xt[m][1], q[1], sum[m]);
+                    } else {
+                        const int at = (g * MT + m) % kBuf, then = (at + 1) % kBuf, tm = (m + MT - kBehind) % MT;
+                        const float ts = m >= kBehind ? sc : sc_last;
+                        sum[at] = mfma32(xt[m][0], q[0], zero);
+                        add(tm, ts, sum[then], 0);
+                        sum[at] = mfma32(xt[m][1], q[1], sum[at]);
+                        add(tm, ts, sum[then], 8);
+                        pin(acc[tm]);
+                    }
+                    read_x(x_buf(g < G - 1 ? s : s + 1), (g + 1) % G, m);
+                    if (ug < 7) {
+                        if (m == 0) next[0] = w.operand(ug + 1, 0, mask);
+                        if (m == MT / 2) next[1] = w.operand(ug + 1, 1, mask);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (ug < 7) q[0] = next[0], q[1] = next[1];
+                sc_last = sc;
+                pin(sc_last);
+            }
+        }
+        if constexpr (kMins) {
+            Terms mn = w.minimums();
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                if (!AL && 4 * u + t >= pairs) mn.r[t] = 0;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const Terms ms = __builtin_bit_cast(Terms, *reinterpret_cast<const u4*>(&gs[u % 2][m][h][n][0]));
+                if constexpr (kWholeBlock) {
+                    const f16v low = mfma32(ms, mn, zero);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[m][r] = fmaf(w.d, sum[m][r], fmaf(-w.dmin, low[r], acc[m][r]));
+                    pin(acc[m]);
+                } else {
+                    acc[m] = mfma32(ms, mn, acc[m]);
+                }
+            }
+        }
+    }
+    if constexpr (!kWholeBlock) {
+#pragma unroll
+        for (int i = 1; i <= kBehind; ++i) {
+            const int m = MT - 1 - kBehind + i, at = i % kBuf;  // the last products' places, as the step's count is 0 mod kBuf
+            add(m, sc_last, sum[at], 0);
+            add(m, sc_last, sum[at], 8);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load outlives the loop
+    float* y = a.partials ? a.partials + (int64_t)split * a.batch * a.out_dim : a.y;
+    const bool whole = b0 + 32 * MT <= a.batch && row0 + 32 <= a.out_dim;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f4 f = *reinterpret_cast<const f4*>(&scales[32 * m + 8 * i + 4 * h]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int b = b0 + 32 * m + 8 * i + 4 * h + r;
+                if (whole || (b < a.batch && row0 + n < a.out_dim))
+                    y[(int64_t)b * a.out_dim + row0 + n] = acc[m][4 * i + r] * f[r];
+            }
+        }
+    }
+}
+
+// Activations for the wide tile form: fp16 in the operands' order, [32 rows][group]
+// of 2 KB, in it [p][h][row] 16 bytes, and each group's sum as two fp16 numbers,
+// [32 rows][unit][2][row][group].  Rows and groups past the end are 0.  A thread
+// converts one group of a row.
+__global__ __launch_bounds__(256) void matmul_fp8_convert_kernel(const uint8_t* x, uint8_t* xf, _Float16* sums, int in_dim,
                                                                  int batch, int units) {
-    const int n = threadIdx.x & 15, g = threadIdx.x >> 4;
+    const int n = threadIdx.x & 31, g = threadIdx.x >> 5;
     const int64_t tile = blockIdx.x / units;
     const int u = blockIdx.x % units;
-    const int64_t row = tile * 16 + n;
+    const int64_t row = tile * 32 + n;
     const int k = u * 256 + g * 32;
     u4 lo = {0, 0, 0, 0}, hi = lo;
     if (row < batch && k < in_dim) {
@@ -725,20 +977,21 @@ __global__ __launch_bounds__(128) void matmul_fp8_convert_kernel(const uint8_t* 
         lo = *reinterpret_cast<const u4*>(p);
         hi = *reinterpret_cast<const u4*>(p + 16);
     }
-    uint8_t* to = xf + ((tile * units + u) * 8 + g) * 1024 + n * 16;
+    uint8_t* to = xf + ((tile * units + u) * 8 + g) * 2048 + n * 16;
     float total = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const Terms t = x_terms(lo[j], hi[j]);
-        *reinterpret_cast<u4*>(to + j * 256) = __builtin_bit_cast(u4, t);
+        *reinterpret_cast<u4*>(to + (j % 2 * 2 + j / 2) * 512) = __builtin_bit_cast(u4, t);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             total = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, t.r[i]), h2{1.f16, 1.f16}, total, false);
     }
     if (sums) {
-        _Float16* s = sums + (tile * units + u) * 256 + n * 8 + g;
-        s[0] = (_Float16)total;
-        s[128] = (_Float16)(total - (float)s[0]);
+        _Float16* s = sums + (tile * units + u) * 512 + n * 8 + g;
+        const _Float16 first = (_Float16)total;
+        s[0] = first;
+        s[256] = (_Float16)(total - (float)first);
     }
 }
 
@@ -751,39 +1004,26 @@ __global__ __launch_bounds__(256) void add_splits_kernel(const float* part, floa
     }
 }
 
-// Converted activations of 16 rows take 8 KB a unit and 512 bytes of sums.  A call keeps at most 1 GB of them: more rows
-// are multiplied piece by piece, each of many more workgroups than the chip holds.
-constexpr int64_t kConverted = 8192 + 512;
-int64_t converted_rows(int units) { return std::max<int64_t>(1, (1 << 30) / (units * kConverted) / 8) * 128; }
+// Rows of a launch, which holds fewer than 2^32 threads: very large batches take several (and no splits).
+int64_t launch_rows(int64_t others, int rows) { return std::max<int64_t>(1, (1 << 21) / others) * rows; }
 
-template <int WT, int MT, int NT, int WN, int G, bool PRE>
-hipError_t launch_tile(MatmulFp8Args a, int splits, hipStream_t stream) {
-    const bool aligned = a.in_dim % 256 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
-    const int units = (a.in_dim + 255) / 256;
-    a.units_per_split = (units + splits - 1) / splits;
+void add_splits(const MatmulFp8Args& a, int splits, hipStream_t stream) {
+    const int64_t n = (int64_t)a.batch * a.out_dim;
+    hipLaunchKernelGGL(add_splits_kernel, dim3((uint32_t)std::min<int64_t>((n + 255) / 256, 2048)), dim3(256), 0, stream,
+                       a.partials, a.y, n, splits);
+}
+
+// The tile forms: `rows` x `cols` a workgroup, `launch` of them a piece of the batch.
+template <class Launch>
+hipError_t launch_tiles(MatmulFp8Args a, int splits, int rows, int cols, int64_t most_rows, hipStream_t stream, Launch launch) {
+    a.units_per_split = ((a.in_dim + 255) / 256 + splits - 1) / splits;
     if (splits == 1) a.partials = nullptr;
-    const int64_t tiles_n = ((int64_t)a.out_dim + 16 * NT * WN - 1) / (16 * NT * WN);
-    // A launch holds fewer than 2^32 threads: very large batches take several (and no splits).
-    int64_t most_rows = std::max<int64_t>(1, (1 << 21) / std::max<int64_t>(tiles_n, PRE ? units : 1)) * (16 * MT);
-    if (PRE) most_rows = std::min(most_rows, converted_rows(units));
+    const int64_t tiles_n = ((int64_t)a.out_dim + cols - 1) / cols;
+    most_rows = std::min(most_rows, launch_rows(tiles_n, rows));
     for (int64_t left = a.batch; left > 0; left -= most_rows) {
         a.batch = (int32_t)std::min(left, most_rows);
-        if constexpr (PRE) {
-            const int64_t row_tiles = (a.batch + 16 * MT - 1) / (16 * MT) * MT;
-            a.sums = Unit<WT>::kMins ? a.xf + row_tiles * units * 8192 : nullptr;
-            hipLaunchKernelGGL(matmul_fp8_convert_kernel, dim3((uint32_t)(row_tiles * units)), dim3(128), 0, stream, a.x, a.xf,
-                               reinterpret_cast<_Float16*>(a.sums), a.in_dim, a.batch, units);
-        }
-        const uint32_t grid = (uint32_t)(tiles_n * ((a.batch + 16 * MT - 1) / (16 * MT)) * splits);
-        if (aligned)
-            hipLaunchKernelGGL((matmul_fp8_tile_kernel<WT, MT, NT, WN, G, PRE, true>), dim3(grid), dim3(64 * WN), 0, stream, a);
-        else
-            hipLaunchKernelGGL((matmul_fp8_tile_kernel<WT, MT, NT, WN, G, PRE, false>), dim3(grid), dim3(64 * WN), 0, stream, a);
-        if (splits > 1) {
-            const int64_t n = (int64_t)a.batch * a.out_dim;
-            hipLaunchKernelGGL(add_splits_kernel, dim3((uint32_t)std::min<int64_t>((n + 255) / 256, 2048)), dim3(256), 0,
-                               stream, a.partials, a.y, n, splits);
-        }
+        launch(a, dim3((uint32_t)(tiles_n * ((a.batch + rows - 1) / rows) * splits)));
+        if (splits > 1) add_splits(a, splits, stream);
         a.x += (int64_t)a.batch * a.in_dim;
         a.x_scale += a.batch;
         a.y += (int64_t)a.batch * a.out_dim;
@@ -791,12 +1031,47 @@ hipError_t launch_tile(MatmulFp8Args a, int splits, hipStream_t stream) {
     return hipGetLastError();
 }
 
+bool wide_loads(const MatmulFp8Args& a) { return a.in_dim % 256 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0; }
+
+template <int WT, int MT, int WN>
+hipError_t launch_tile(const MatmulFp8Args& all, int splits, hipStream_t stream) {
+    return launch_tiles(all, splits, 16 * MT, 16 * WN, all.batch, stream, [&](const MatmulFp8Args& a, dim3 grid) {
+        if (wide_loads(a))
+            hipLaunchKernelGGL((matmul_fp8_tile_kernel<WT, MT, WN, true>), grid, dim3(64 * WN), 0, stream, a);
+        else
+            hipLaunchKernelGGL((matmul_fp8_tile_kernel<WT, MT, WN, false>), grid, dim3(64 * WN), 0, stream, a);
+    });
+}
+
+// Converted activations of 32 rows take 16 KB a unit and 1 KB of sums.  A call keeps at most 1 GB of them: more rows
+// are multiplied piece by piece, each of many more workgroups than the chip holds.
+constexpr int64_t kConverted = 16384 + 1024;
+int64_t converted_rows(int units) {
+    return std::max<int64_t>(1, (1 << 30) / (units * kConverted) / (kWideRows / 32)) * kWideRows;
+}
+
+template <int WT>
+hipError_t launch_wide(const MatmulFp8Args& all, int splits, hipStream_t stream) {
+    const int units = (all.in_dim + 255) / 256;
+    const int64_t most = std::min(converted_rows(units), launch_rows(units, kWideRows));
+    return launch_tiles(all, splits, kWideRows, 32 * kWideWaves, most, stream, [&](MatmulFp8Args a, dim3 grid) {
+        const int64_t tiles = ((int64_t)a.batch + kWideRows - 1) / kWideRows * (kWideRows / 32);
+        a.sums = Unit<WT>::kMins ? a.xf + tiles * units * 16384 : nullptr;
+        hipLaunchKernelGGL(matmul_fp8_convert_kernel, dim3((uint32_t)(tiles * units)), dim3(256), 0, stream, a.x, a.xf,
+                           reinterpret_cast<_Float16*>(a.sums), a.in_dim, a.batch, units);
+        if (wide_loads(a))
+            hipLaunchKernelGGL((matmul_fp8_wide_kernel<WT, true>), grid, dim3(64 * kWideWaves), 0, stream, a);
+        else
+            hipLaunchKernelGGL((matmul_fp8_wide_kernel<WT, false>), grid, dim3(64 * kWideWaves), 0, stream, a);
+    });
+}
+
 template <int WT>
 hipError_t launch_type(const MatmulFp8Args& a, const MatmulFp8Plan& p, hipStream_t stream) {
     switch (p.form) {
-        case MatmulFp8Plan::kTile128: return launch_tile<WT, 8, 2, 8, 4, true>(a, p.splits, stream);
-        case MatmulFp8Plan::kTile64: return launch_tile<WT, 4, 1, 8, 4, false>(a, p.splits, stream);
-        case MatmulFp8Plan::kTile32: return launch_tile<WT, 2, 1, 4, 4, false>(a, p.splits, stream);
+        case MatmulFp8Plan::kWide: return launch_wide<WT>(a, p.splits, stream);
+        case MatmulFp8Plan::kTile64: return launch_tile<WT, 4, 8>(a, p.splits, stream);
+        case MatmulFp8Plan::kTile32: return launch_tile<WT, 2, 4>(a, p.splits, stream);
         default: break;
     }
     // The stream form.  With many outputs two tiles share a workgroup's activations; with few, more waves share a tile's
@@ -835,7 +1110,7 @@ MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, in
         double around;  // a round's time before and behind its units
     };
     // Measured on 3584 and 18944 of K, Q4_0, at 65 to 2048 rows.
-    constexpr Form kForms[] = {{MatmulFp8Plan::kTile128, 128, 256, {4.85, 0, 0, 0}, 10},
+    constexpr Form kForms[] = {{MatmulFp8Plan::kWide, kWideRows, 32 * kWideWaves, {4.3, 0, 0, 0}, 10},
                                {MatmulFp8Plan::kTile64, 64, 128, {2.05, 3.7, 0, 0}, 4},
                                {MatmulFp8Plan::kTile32, 32, 64, {1.33, 1.75, 2.5, 3.25}, 4}};
     const int units = (in_dim + 255) / 256;
@@ -866,9 +1141,9 @@ MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, in
 }
 
 int64_t matmul_fp8_x_bytes(int32_t in_dim, int32_t batch, const MatmulFp8Plan& plan) {
-    if (plan.form != MatmulFp8Plan::kTile128) return 0;
+    if (plan.form != MatmulFp8Plan::kWide) return 0;
     const int units = (in_dim + 255) / 256;
-    return (std::min<int64_t>(batch, converted_rows(units)) + 127) / 128 * 8 * units * kConverted;
+    return (std::min<int64_t>(batch, converted_rows(units)) + kWideRows - 1) / kWideRows * (kWideRows / 32) * units * kConverted;
 }
 
 int64_t matmul_fp8_row_bytes(int32_t w_type, int32_t in_dim) {
