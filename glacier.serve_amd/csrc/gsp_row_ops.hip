@@ -7,6 +7,13 @@
 // once and every output written once, with the row's two reductions (the sum
 // of squares, then the largest magnitude) between.  Rows past what a
 // workgroup's registers hold (kRowMax values) are read again for each pass.
+//
+// Bound by memory where there is enough of it: 8193 rows of 4096 with a residual
+// and all three results 112 us, 5.1 TB/s (a large copy reaches 4.8); 4099 rows of
+// 3584 into codes 11.8 us, 6.2 TB/s (the inputs lie in the last-level cache); 64
+// rows of 18944, gated, 4.5 us on the GPU, 2.2 TB/s (64 of 256 CUs).  A step's small
+// rows are bound by the launch: 8 rows of 896 take 2.8 us on the GPU, 64 of 3584
+// 3.8, and a call 3.4 us on the host.
 #include "gsp_internal.h"
 #include "../../include/glacier_paged.h"
 
