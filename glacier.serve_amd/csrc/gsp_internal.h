@@ -242,7 +242,8 @@ struct MatmulFp8Plan {
     int32_t splits = 1;
     int32_t cus = 1;
 };
-MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, int cus);
+// aligned: rows of weights are whole units of 256, 16-byte aligned.
+MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, bool aligned, int cus);
 int64_t matmul_fp8_x_bytes(int32_t in_dim, int32_t batch, const MatmulFp8Plan& plan);
 int64_t matmul_fp8_row_bytes(int32_t w_type, int32_t in_dim);
 hipError_t launch_matmul_fp8(int32_t w_type, const MatmulFp8Args& a, const MatmulFp8Plan& plan, hipStream_t stream);

@@ -386,10 +386,13 @@ int even_waves(int units, int most) {
     return (units + per - 1) / per;
 }
 
+// Rows of weights are whole units and 16-byte aligned.
+bool wide_loads(const MatmulFp8Args& a) { return a.in_dim % 256 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0; }
+
 template <int WT, int MT, int R, int NT, int W>
 hipError_t launch_form(MatmulFp8Args a, hipStream_t stream) {
     const int waves = even_waves((a.in_dim + 255) / 256, W);
-    const bool aligned = a.in_dim % 256 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
+    const bool aligned = wide_loads(a);
     // A launch holds fewer than 2^32 threads: very large batches take several.
     const int64_t tiles = ((int64_t)a.out_dim + 16 * NT - 1) / (16 * NT);
     const int64_t most_rows = std::max<int64_t>(1, (1 << 21) / tiles) * (4 * R * MT);
@@ -749,6 +752,127 @@ __device__ inline f16v mfma32(const Terms& a, const Terms& b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
 
+// The stream form of more rows: 32 weight rows by 32 batch rows a workgroup, in the
+// 32 x 32 x 16 instruction, its waves sharing the units of K as above.  A lane's
+// activations of a group are two pieces of 8 bytes of its row, which LDS gives it as
+// they are.  A unit's sums of x by group are products as well, with ones in row g for
+// group g: they arrive as [group][batch row], four groups a lane half, and meet the
+// minimums as two fp16 numbers each in one product.  Rows of weights are whole units,
+// 16-byte aligned.  us, 64 rows of 18944 x 3584: Q4_0 23.3, Q4_1 25.5, Q4_K 24.9, with
+// 16 x 16 x 32 products 26.7, 33.3 and 31.9: fewer of them, no swaps of activations, and
+// minimums and Q4_K's scales without the vector unit, whose issue bounds both.
+template <int WT, int W>
+__global__ __launch_bounds__(64 * W) void matmul_fp8_stream32_kernel(MatmulFp8Args a) {
+    constexpr int kRow = Unit<WT>::kRow, kTile = 32 * kRow, kX = 32 * 256, kSlot = kTile + kX;
+    constexpr int kWide = kTile / 1024 * 1024;  // of the weights, loaded 16 bytes a lane
+    constexpr bool kMins = Unit<WT>::kMins, kWholeBlock = WT == GSP_WTYPE_Q4_K;
+    static_assert(kSlot >= 4096, "the partial sums take the slots' place");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[W * kSlot];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int n = lane & 31, h = lane >> 5;
+    const int tiles_b = (a.batch + 31) / 32;
+    const int row0 = blockIdx.x / tiles_b * 32, b0 = blockIdx.x % tiles_b * 32;
+    const int units = a.in_dim >> 8;
+    uint8_t* slot = lds + wave * kSlot;
+
+    const auto weight_at = [&](int byte, int u) {
+        const int r = byte / kRow, c = byte % kRow;
+        const int64_t row = (int64_t)min(row0 + r, a.out_dim - 1) * a.row_bytes;
+        return static_cast<const uint8_t*>(a.w) + row + (int64_t)u * kRow + c;
+    };
+    // Piece p (16 bytes) of row r of activations goes to place p ^ r of the row, so that the reads below spread over the
+    // banks.
+    const auto send = [&](int u) {
+#pragma unroll
+        for (int at = 0; at < kWide; at += 1024) load_to_lds<16>(weight_at(at + 16 * lane, u), slot + at);
+#pragma unroll
+        for (int at = kWide; at < kTile; at += 256) load_to_lds<4>(weight_at(at + 4 * lane, u), slot + at);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + (lane >> 4), p = (lane & 15) ^ (r & 15);
+            const int64_t row = (int64_t)min(b0 + r, a.batch - 1) * a.in_dim;
+            load_to_lds<16>(a.x + row + u * 256 + p * 16, slot + kTile + i * 1024);
+        }
+    };
+
+    const f16v zero = {};
+    f16v acc = zero, sum[2] = {zero, zero};
+    float sc_last = 0.f;
+    uint32_t mask = kNib;
+    asm volatile("" : "+v"(mask));
+    if (wave < units) send(wave);
+    for (int u = wave; u < units; u += waves) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the unit has landed
+        Rows<WT> w;
+        w.read(slot, n, h);
+        u2 x[8][2];
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                x[g][i] = *reinterpret_cast<const u2*>(slot + kTile + n * 256 + ((2 * g + i) ^ (n & 15)) * 16 + 8 * h);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and is in registers: the slot may be overwritten
+        if (u + waves < units) send(u + waves);
+        f16v sx = zero;
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+            Terms xt[2];
+#pragma unroll
+            for (int p = 0; p < 2; ++p) xt[p] = x_terms(x[g][0][p], x[g][1][p]);
+            const int at = kWholeBlock ? 0 : g % 2;
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+                sum[at] = mfma32(xt[p], w.operand(g, p, mask), p || (kWholeBlock && g) ? sum[at] : zero);
+            if constexpr (kMins) {
+                const Terms ones = splat_terms(n == g ? 0x3c00u : 0u);
+#pragma unroll
+                for (int p = 0; p < 2; ++p) sx = mfma32(ones, xt[p], sx);
+            }
+            if constexpr (!kWholeBlock) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[r] = fmaf(sc_last, sum[1 - at][r], acc[r]);
+                sc_last = w.scale(g);
+            }
+        }
+        if constexpr (kMins) {
+            Terms mn = w.minimums(), ms;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float s0 = sx[2 * i], s1 = sx[2 * i + 1];
+                const h2 first = {(_Float16)s0, (_Float16)s1};
+                const h2 rest = {(_Float16)(s0 - (float)first[0]), (_Float16)(s1 - (float)first[1])};
+                ms.r[i] = __builtin_bit_cast(uint32_t, first);
+                ms.r[2 + i] = __builtin_bit_cast(uint32_t, rest);
+                mn.r[i] = h ? mn.r[2 + i] : mn.r[i];
+                mn.r[2 + i] = mn.r[i];
+            }
+            if constexpr (kWholeBlock) {
+                const f16v low = mfma32(ms, mn, zero);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[r] = fmaf(w.d, sum[0][r], fmaf(-w.dmin, low[r], acc[r]));
+            } else {
+                acc = mfma32(ms, mn, acc);
+            }
+        }
+    }
+    if constexpr (!kWholeBlock) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[r] = fmaf(sc_last, sum[1][r], acc[r]);
+    }
+    __syncthreads();  // every wave is done with its slots
+    float* part = reinterpret_cast<float*>(lds);  // [waves][16][lane]
+#pragma unroll
+    for (int r = 0; r < 16; ++r) part[(wave * 16 + r) * 64 + lane] = acc[r];
+    __syncthreads();
+    for (int e = threadIdx.x; e < 1024; e += blockDim.x) {
+        float s = 0.f;
+        for (int v = 0; v < waves; ++v) s += part[v * 1024 + e];
+        const int r = e >> 6, b = b0 + (r & 3) + 8 * (r >> 2) + 4 * (e >> 5 & 1), o = row0 + (e & 31);
+        if (b < a.batch && o < a.out_dim) a.y[(int64_t)b * a.out_dim + o] = s * a.x_scale[b];
+    }
+}
+
 // The wide tile form: 128 batch rows by 256 weight rows a workgroup, 128 by 32 a wave,
 // in the 32 x 32 x 16 instruction, of which half as many are issued for the same terms.
 // Beside a multiply-add for each output it takes 9.3 ns a SIMD for 16 x 16 x 32 terms,
@@ -1004,6 +1128,13 @@ __global__ __launch_bounds__(256) void add_splits_kernel(const float* part, floa
     }
 }
 
+template <int WT, int W>
+hipError_t launch_stream32(const MatmulFp8Args& a, hipStream_t stream) {
+    const uint32_t grid = (uint32_t)((a.out_dim + 31) / 32 * ((a.batch + 31) / 32));
+    hipLaunchKernelGGL((matmul_fp8_stream32_kernel<WT, W>), dim3(grid), dim3(64 * even_waves(a.in_dim / 256, W)), 0, stream, a);
+    return hipGetLastError();
+}
+
 // Rows of a launch, which holds fewer than 2^32 threads: very large batches take several (and no splits).
 int64_t launch_rows(int64_t others, int rows) { return std::max<int64_t>(1, (1 << 21) / others) * rows; }
 
@@ -1030,8 +1161,6 @@ hipError_t launch_tiles(MatmulFp8Args a, int splits, int rows, int cols, int64_t
     }
     return hipGetLastError();
 }
-
-bool wide_loads(const MatmulFp8Args& a) { return a.in_dim % 256 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0; }
 
 template <int WT, int MT, int WN>
 hipError_t launch_tile(const MatmulFp8Args& all, int splits, hipStream_t stream) {
@@ -1084,8 +1213,17 @@ hipError_t launch_type(const MatmulFp8Args& a, const MatmulFp8Plan& p, hipStream
         return wide ? launch_form<WT, 1, 2, 2, 8>(a, stream) : launch_form<WT, 1, 2, 1, 16>(a, stream);
     if (a.batch <= 16)
         return wide ? launch_form<WT, 1, 4, 2, 8>(a, stream) : launch_form<WT, 1, 4, 1, 8>(a, stream);
-    // More rows: 32 a workgroup while its workgroups, one a CU, run in one round (18944 x 3584 at 32 rows 19.5 us with
-    // one tile; at 64 rows 27.6 with two); else 16 a workgroup (3584 x 4608 at 37 rows 10.2, 13 with 32).
+    // More rows, in 32 x 32 tiles where these fill more than half of the CUs: in one round with 8 waves each (3584 x 4608
+    // at 32 rows Q4_0 8.2 against 9.3, Q4_K 8.4 and 10.4; 3584 x 3584, on 112 CUs, 8.2 and 7.5), in several with 4, three
+    // a CU (Q4_0 4096 x 14336 at 32 rows 14.6 against 17.5, at 64 24.6 and 28.2), unless a second round would be short and
+    // much of the last rows' tile is empty (3584 x 4608 at 37 rows 14.1 and 11.3, 3584 x 8192 15.0 and 15.2).
+    const int64_t tiles = ((int64_t)a.out_dim + 31) / 32 * ((a.batch + 31) / 32);
+    if (a.batch <= 64 && wide_loads(a) && tiles > p.cus / 2) {
+        if (tiles <= p.cus) return launch_stream32<WT, 8>(a, stream);
+        if (a.batch <= 32 || a.batch > 48 || tiles >= 2 * p.cus) return launch_stream32<WT, 4>(a, stream);
+    }
+    // Otherwise 32 rows a workgroup while its workgroups, one a CU, run in one round (18944 x 3584 at 32 rows 18.9 us with
+    // one tile); else 16 a workgroup (3584 x 4608 at 37 rows 11.3, 13 with 32).
     const int64_t tiles_b = (a.batch + 31) / 32;
     if (a.out_dim >= 16384 && a.batch <= 32) return launch_form<WT, 2, 4, 2, 4>(a, stream);
     if ((a.out_dim + 15) / 16 * tiles_b <= p.cus) return launch_form<WT, 2, 4, 1, 8>(a, stream);
@@ -1099,7 +1237,7 @@ hipError_t launch_type(const MatmulFp8Args& a, const MatmulFp8Plan& p, hipStream
 // workgroup takes a time per unit of K that depends on how many share its CU;
 // workgroups run in rounds of what the chip holds; splits of K add the partial
 // sums' traffic and a launch.
-MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, int cus) {
+MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, bool aligned, int cus) {
     MatmulFp8Plan best{};
     best.cus = cus;
     // Tile offsets are 32-bit; a longer K is streamed.  Up to 64 rows only wide outputs repay the conversion.
@@ -1115,6 +1253,12 @@ MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, in
                                {MatmulFp8Plan::kTile32, 32, 64, {1.33, 1.75, 2.5, 3.25}, 4}};
     const int units = (in_dim + 255) / 256;
     double least = 0;
+    if (batch <= 64 && aligned) {
+        // The stream's 32 x 32 tiles, three a CU: 3584 x 18944 at 48 rows 27.7 us against 31.9 in tiles of 64, 4096 x 32768
+        // 43.7 and 37.4, 1024 x 65536 33 and 20.
+        const double tiles = (double)(((int64_t)out_dim + 31) / 32 * ((batch + 31) / 32));
+        least = 7 + tiles / (3 * cus) * (1.2 + 0.86 * units);
+    }
     for (const Form& f : kForms) {
         if (batch <= f.rows / 2) continue;  // half of it empty: the next one takes less, and no workspace up to 64 rows
         const double tiles = (double)(((int64_t)batch + f.rows - 1) / f.rows) * (((int64_t)out_dim + f.cols - 1) / f.cols);

@@ -1171,7 +1171,8 @@ int gsp_matmul_batch_fp8(gsp_ctx* ctx, int32_t w_type, const void* w_dev, const 
         return gsp::fail(GSP_E_INVALID_ARG, "y overlaps another argument");
     int rc = set_device(ctx);
     if (rc) return rc;
-    const gsp::MatmulFp8Plan plan = gsp::plan_matmul_fp8(in_dim, out_dim, batch, std::max(1, ctx->num_cus));
+    const gsp::MatmulFp8Plan plan = gsp::plan_matmul_fp8(in_dim, out_dim, batch, in_dim % 256 == 0 && is_aligned(w_dev, 16),
+                                                        std::max(1, ctx->num_cus));
     MatmulNeeds need;
     if (plan.splits > 1) need.partials = (size_t)plan.splits * batch * out_dim;
     need.x = (size_t)gsp::matmul_fp8_x_bytes(in_dim, batch, plan) / sizeof(uint16_t);

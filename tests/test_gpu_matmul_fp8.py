@@ -129,3 +129,32 @@ def test_weights_at_four_byte_addresses(torch_mod, ctx):
                                  out_dim, batch)
             ctx.sync()
             assert np.all(np.abs(y.cpu().numpy() - want) <= bound + 1e-40)
+
+
+# 17 to 64 rows in tiles of 32 by 32: one round of workgroups, several, ragged rows and outputs, K of one unit and of
+# many; the last two are wide enough that the tile forms are weighed against them.
+STREAM32 = [(256, 4500, 17), (1024, 4611, 31), (2560, 3590, 37), (4864, 4100, 32), (512, 8300, 40), (768, 5000, 64),
+            (256, 16411, 32), (512, 17000, 50), (256, 33000, 64)]
+
+
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("shape", STREAM32, ids=lambda s: f"in{s[0]}_out{s[1]}_b{s[2]}")
+def test_tiles_of_32_rows_that_share_k(torch_mod, ctx, shape, name):
+    test_matches_64_bits(torch_mod, ctx, shape, name)
+
+
+@pytest.mark.parametrize("name", list(TYPES))
+def test_nan_rows_in_tiles_of_32(torch_mod, ctx, name):
+    torch = torch_mod
+    rng = np.random.default_rng(3)
+    in_dim, out_dim, batch = 512, 4500, 29
+    raw, codes, scale = _inputs(rng, TYPES[name], in_dim, out_dim, batch)
+    codes[1, 511], codes[7, 0], codes[28, 300] = 0x7f, 0xff, 0x7f
+    wd, xd, sd = (torch.from_numpy(a).cuda() for a in (raw, codes, scale))
+    y = torch.zeros((batch, out_dim), device="cuda")
+    torch.cuda.synchronize()
+    ctx.matmul_batch_fp8(TYPES[name], wd.data_ptr(), xd.data_ptr(), sd.data_ptr(), y.data_ptr(), in_dim, out_dim, batch)
+    ctx.sync()
+    bad = torch.isnan(y)
+    assert set(np.nonzero(bad.any(1).cpu().numpy())[0]) == {1, 7, 28}
+    assert bad[[1, 7, 28]].all()
