@@ -703,13 +703,15 @@ struct Rows {
             }
         }
     }
+    // Quants of group g times 1 / kCode (Q4_0, Q4_1).
+    __device__ inline Terms quants(int g, int p, uint32_t mask) const {
+        const uint32_t a = q[2 * g + p];
+        return Terms{{(a << 4) & mask, (a >> 4) & mask, a & mask, (a >> 8) & mask}};
+    }
     // The p-th operand of group g: q - 8 (Q4_0) and q times the group's 6-bit scale, an exact integer up to 945 (Q4_K),
     // formed from 1024 + 16 q in one fused step, or q times 1 / kCode (Q4_1).  mask: kNib in a register.
     __device__ inline Terms operand(int g, int p, uint32_t mask) const {
-        if constexpr (WT == GSP_WTYPE_Q4_1) {
-            const uint32_t a = q[2 * g + p];
-            return Terms{{(a << 4) & mask, (a >> 4) & mask, a & mask, (a >> 8) & mask}};
-        }
+        if constexpr (WT == GSP_WTYPE_Q4_1) return quants(g, p, mask);
         h2 f = {0.0625f16, 0.0625f16}, c = {-72.f16, -72.f16};
         if constexpr (WT == GSP_WTYPE_Q4_K) {
             const float sc = (float)((s[g / 4] >> (8 * (g % 4))) & 0xffu) * 0.0625f;
@@ -766,6 +768,9 @@ __global__ __launch_bounds__(64 * W) void matmul_fp8_stream32_kernel(MatmulFp8Ar
     constexpr int kRow = Unit<WT>::kRow, kTile = 32 * kRow, kX = 32 * 256, kSlot = kTile + kX;
     constexpr int kWide = kTile / 1024 * 1024;  // of the weights, loaded 16 bytes a lane
     constexpr bool kMins = Unit<WT>::kMins, kWholeBlock = WT == GSP_WTYPE_Q4_K;
+    // Q4_0's sums start at -8 / kCode times the sum of x: two products instead of eight instructions an operand.
+    constexpr bool kStart = WT == GSP_WTYPE_Q4_0;
+    constexpr float kOut = kStart ? kCode : 1.f;
     static_assert(kSlot >= 4096, "the partial sums take the slots' place");
     __shared__ __attribute__((aligned(16))) uint8_t lds[W * kSlot];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
@@ -821,9 +826,16 @@ __global__ __launch_bounds__(64 * W) void matmul_fp8_stream32_kernel(MatmulFp8Ar
 #pragma unroll
             for (int p = 0; p < 2; ++p) xt[p] = x_terms(x[g][0][p], x[g][1][p]);
             const int at = kWholeBlock ? 0 : g % 2;
+            if constexpr (kStart) {
 #pragma unroll
-            for (int p = 0; p < 2; ++p)
-                sum[at] = mfma32(xt[p], w.operand(g, p, mask), p || (kWholeBlock && g) ? sum[at] : zero);
+                for (int p = 0; p < 2; ++p) sum[at] = mfma32(xt[p], splat_terms(kMinus8), p ? sum[at] : zero);
+#pragma unroll
+                for (int p = 0; p < 2; ++p) sum[at] = mfma32(xt[p], w.quants(g, p, mask), sum[at]);
+            } else {
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+                    sum[at] = mfma32(xt[p], w.operand(g, p, mask), p || (kWholeBlock && g) ? sum[at] : zero);
+            }
             if constexpr (kMins) {
                 const Terms ones = splat_terms(n == g ? 0x3c00u : 0u);
 #pragma unroll
@@ -869,7 +881,7 @@ __global__ __launch_bounds__(64 * W) void matmul_fp8_stream32_kernel(MatmulFp8Ar
         float s = 0.f;
         for (int v = 0; v < waves; ++v) s += part[v * 1024 + e];
         const int r = e >> 6, b = b0 + (r & 3) + 8 * (r >> 2) + 4 * (e >> 5 & 1), o = row0 + (e & 31);
-        if (b < a.batch && o < a.out_dim) a.y[(int64_t)b * a.out_dim + o] = s * a.x_scale[b];
+        if (b < a.batch && o < a.out_dim) a.y[(int64_t)b * a.out_dim + o] = s * kOut * a.x_scale[b];
     }
 }
 
