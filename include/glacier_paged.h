@@ -285,7 +285,8 @@ int gsp_mrope_write_step(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, int32_t n_
  * y's codes and each row's scale max(max |y|, 2^-100) / 448, every code the
  * e4m3 value nearest to y / scale.  A row that holds a NaN gets NaN codes or a
  * NaN scale; one that holds an infinity gets a NaN or zero for every value, as
- * the formula does.  sum_dev and y_dev may each be x_dev or residual_dev
+ * the formula does.  Squares and their sum are fp32: where they overflow (values
+ * past 2^63) a row becomes 0.  sum_dev and y_dev may each be x_dev or residual_dev
  * itself; every other overlap of an output with another argument is refused
  * (GSP_E_INVALID_ARG).  eps is finite and >= 0.  rows may be 0; dim is at least
  * 1.  Rows of any length and 4-byte alignment are taken; 16-byte aligned
@@ -296,7 +297,8 @@ int gsp_rms_norm(gsp_ctx* ctx, int32_t rows, int32_t dim, const float* x_dev, co
 
 /* Rows of fp32 activations into codes and scales (as y's of gsp_rms_norm).
  * GSP_ACT_NONE quantises a_dev (b_dev NULL), GSP_ACT_SILU_MUL
- * a / (1 + exp(-a)) * b.  Row i starts at a_dev + i * stride (and b_dev + i *
+ * a / (1 + exp(-a)) * b, where the quotient's 1 / (1 + exp(-a)) counts as 0 below
+ * 2^-126 (a < -87.3).  Row i starts at a_dev + i * stride (and b_dev + i *
  * stride), stride >= dim in floats, so that the halves of one fused gate and up
  * projection are given as they lie; the codes are dense, [rows][dim].  The
  * outputs must not overlap the inputs or each other. */
@@ -316,13 +318,14 @@ int gsp_quantize_fp8(gsp_ctx* ctx, int32_t act, int32_t rows, int32_t dim, int64
  * Products of codes and quants are exact and sums are fp32: no rounding of x or
  * W is added to the codes' own.  in_dim is a multiple of 64 (256 for Q4_K)
  * and out_dim at most 2^24 (GSP_E_UNSUPPORTED otherwise, as for other weight
- * types).  Results are the same bit for bit on every call of the same sizes, captured or not; the number
- * of rows may change the order of an output's sums.
- * Graph capture is as for gsp_matmul_batch: products of more than 64 rows may
- * need a workspace, so run the product, or a larger one, once before capturing
- * it (GSP_E_STATE otherwise, and nothing is enqueued); captured products keep
- * buffers of their own and their graphs must not run at the same time as each
- * other.  Up to 64 rows nothing is needed; above, at most about 1 GB. */
+ * types).  Results are the same bit for bit on every call of the same sizes and
+ * 16-byte alignment of W, captured or not; the number of rows and the alignment
+ * may change the order of an output's sums.
+ * Graph capture: products of more than 64 rows may need a workspace of up to about
+ * 1 GB, so run the product itself once before capturing it (a larger one may take a
+ * form that needs none; GSP_E_STATE otherwise, and nothing is enqueued).  Captured
+ * products keep buffers of their own, and their graphs must not run at the same time
+ * as each other.  Up to 64 rows nothing is needed. */
 #define GSP_WTYPE_Q4_0 2
 #define GSP_WTYPE_Q4_1 3
 int gsp_matmul_batch_fp8(gsp_ctx* ctx, int32_t w_type, const void* w_dev, const uint8_t* x_dev,
