@@ -892,12 +892,12 @@ __global__ __launch_bounds__(64 * W) void matmul_fp8_stream32_kernel(MatmulFp8Ar
 // The wide tile form: 128 batch rows by 256 weight rows a workgroup, 128 by 32 a wave,
 // in the 32 x 32 x 16 instruction, of which half as many are issued for the same terms.
 // Beside a multiply-add for each output it takes 9.3 ns a SIMD for 16 x 16 x 32 terms,
-// the other one 11.2, and issue is what bounds this form: the vector unit is busy 72 %
-// of the time (Q4_0, 18944 x 3584 at 2048 rows), with 512 multiply-adds, 176
+// the other one 11.2, and issue is what bounds this form: the vector unit is busy 73 %
+// of the time (Q4_0, 3584 x 18944 at 2048 rows), with 512 multiply-adds, 176
 // instructions of expansion, 64 products and 63 others a wave and unit; the matrix unit
-// 45 %.  Activations come converted from matmul_fp8_convert_kernel, as converting them
-// in every workgroup took 4 % longer there.  us at 2048 rows (TFLOP/s), 3584 x 18944
-// and 18944 x 3584: Q4_0 332 (837) and 320, Q4_1 333 and 330, Q4_K 313 and 302.
+// 43 %.  Activations come converted from matmul_fp8_convert_kernel (9 us there), as
+// converting them in every workgroup took 4 % longer.  us at 2048 rows (TFLOP/s), 3584 x
+// 18944 and 18944 x 3584: Q4_0 319 (872) and 307, Q4_1 317 and 310, Q4_K 310 and 298.
 //
 // Measured without gain: the loads to LDS sent one by one between the products, the
 // weights read before their unit begins, activations through registers, the barrier
