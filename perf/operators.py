@@ -253,7 +253,7 @@ def _prepare_mrope(s, case, seed):
     g = _gen(seed)
     s.block = torch.from_numpy(ids[offsets[row] + at // page].astype(np.int64)).cuda()
     s.slot = torch.from_numpy(at % page).cuda()
-    s.axes = torch.from_numpy(np.ascontiguousarray(axes)).cuda()  # [3, tokens], dense: the call takes its address
+    s.axes = torch.from_numpy(axes).cuda()
     shape = (blocks, 2, kvh, page, d)
     dtype = torch.float32 if case["kv"] == "f32" else torch.float16
     s.keys = torch.randn(shape, generator=g, device="cuda").to(dtype)
