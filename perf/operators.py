@@ -266,6 +266,7 @@ def _prepare_mrope(s, case, seed):
         s.q, s.k, s.v = (torch.randn((n, w), generator=g, device="cuda") for w in (wide, kv, kv))
     s.q_out = torch.zeros((n, heads, d), device="cuda")
     if own:
+        s.axes = s.axes.contiguous()  # the call takes the address of dense [3, tokens], which numpy's order need not be
         # The engine packs a tick once for all its layers.
         gsp = _gsp()
         s.ctx = gsp.Context(0)
