@@ -135,7 +135,7 @@ __device__ inline float silu_mul(float g, float u) {
 
 // The row's values before the norm's factor: x + residual, a, or silu(a) b.
 template <int KIND, int VEC>
-__device__ inline Piece<VEC> row_value(const RowArgs& a, const float* x, const float* o, int at) {
+__device__ inline Piece<VEC> row_value(const RowArgs& a, const float* x, const float* o, int64_t at) {
     Piece<VEC> r = load_piece<VEC>(x + at);
     if (KIND == kRowSilu || (KIND == kRowNorm && o)) {
         const Piece<VEC> q = load_piece<VEC>(o + at);
@@ -214,7 +214,8 @@ __global__ __launch_bounds__(1024) void row_kernel(RowArgs a) {
 
 // Rows of more than kRowMax values: each pass reads the row again.  The norm's
 // passes after the first read x + residual, then y, back where the caller keeps
-// them, so that they may overwrite x or the residual.
+// them, so that they may overwrite x or the residual.  A place may be past
+// 2^31 - 1 before the loop ends.
 template <int KIND>
 __global__ __launch_bounds__(1024) void long_row_kernel(RowArgs a) {
     __shared__ float lsum[16];
@@ -225,7 +226,7 @@ __global__ __launch_bounds__(1024) void long_row_kernel(RowArgs a) {
     float f = 1.0f;
     if constexpr (KIND == kRowNorm) {
         float sq = 0.f;
-        for (int at = threadIdx.x; at < a.dim; at += blockDim.x) {
+        for (int64_t at = threadIdx.x; at < a.dim; at += blockDim.x) {
             const float v = row_value<KIND, 1>(a, x, o, at).v[0];
             sq += v * v;
             if (a.sum) a.sum[row * a.dim + at] = v;
@@ -237,7 +238,7 @@ __global__ __launch_bounds__(1024) void long_row_kernel(RowArgs a) {
         f = 1.0f / sqrtf(block_sum(sq, lsum) / (float)a.dim + a.eps);
     }
     uint32_t top = 0;
-    for (int at = threadIdx.x; at < a.dim; at += blockDim.x) {
+    for (int64_t at = threadIdx.x; at < a.dim; at += blockDim.x) {
         float v = row_value<KIND, 1>(a, x, o, at).v[0];
         if constexpr (KIND == kRowNorm) {
             v = v * f * a.weight[at];
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(1024) void long_row_kernel(RowArgs a) {
     float scale, inv;
     row_scale(block_max(top, lmax), &scale, &inv);
     if (threadIdx.x == 0) a.scale[row] = scale;
-    for (int at = threadIdx.x; at < a.dim; at += blockDim.x) {
+    for (int64_t at = threadIdx.x; at < a.dim; at += blockDim.x) {
         Piece<1> r;
         if (KIND == kRowNorm && a.y) {
             r.v[0] = a.y[row * a.dim + at];
