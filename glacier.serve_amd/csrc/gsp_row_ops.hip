@@ -41,7 +41,8 @@ enum { kRowNorm = 0, kRowPlain = 1, kRowSilu = 2 };
 
 // Sum and largest value over the workgroup.  Each wave's result crosses LDS;
 // every thread gets the total.  The order of the sum is fixed.
-__device__ inline float wave_sum(float v) {
+template <typename T>
+__device__ inline T wave_sum(T v) {
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m);
     return v;
@@ -51,13 +52,14 @@ __device__ inline uint32_t wave_max(uint32_t v) {
     for (int m = 32; m >= 1; m >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, m));
     return v;
 }
-__device__ inline float block_sum(float v, float* lds) {
+template <typename T>
+__device__ inline T block_sum(T v, T* lds) {
     v = wave_sum(v);
     const int waves = blockDim.x >> 6;
     if (waves == 1) return v;
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
-    float t = 0.f;
+    T t = 0;
     for (int i = 0; i < waves; ++i) t += lds[i];
     return t;
 }
@@ -215,33 +217,35 @@ __global__ __launch_bounds__(1024) void row_kernel(RowArgs a) {
 // Rows of more than kRowMax values: each pass reads the row again.  The norm's
 // passes after the first read x + residual, then y, back where the caller keeps
 // them, so that they may overwrite x or the residual.  A place may be past
-// 2^31 - 1 before the loop ends.
+// 2^31 - 1 before the loop ends.  A thread adds dim / 1024 squares one after the
+// other: they, their sum and the norm's factor hold 64 bits (in fp32 equal values
+// of 1.1 put y of a row of 2^24 off by 920 steps).
 template <int KIND>
 __global__ __launch_bounds__(1024) void long_row_kernel(RowArgs a) {
-    __shared__ float lsum[16];
+    __shared__ double lsum[16];
     __shared__ uint32_t lmax[16];
     const int64_t row = blockIdx.x;
     const float* x = a.x + row * a.stride;
     const float* o = a.other ? a.other + row * a.stride : nullptr;
-    float f = 1.0f;
+    double f = 1.0;
     if constexpr (KIND == kRowNorm) {
-        float sq = 0.f;
+        double sq = 0;
         for (int64_t at = threadIdx.x; at < a.dim; at += blockDim.x) {
             const float v = row_value<KIND, 1>(a, x, o, at).v[0];
-            sq += v * v;
+            sq += (double)v * v;
             if (a.sum) a.sum[row * a.dim + at] = v;
         }
         if (a.sum) {
             x = a.sum + row * a.dim;  // each thread reads back what it wrote
             o = nullptr;
         }
-        f = 1.0f / sqrtf(block_sum(sq, lsum) / (float)a.dim + a.eps);
+        f = 1.0 / sqrt(block_sum(sq, lsum) / a.dim + a.eps);
     }
     uint32_t top = 0;
     for (int64_t at = threadIdx.x; at < a.dim; at += blockDim.x) {
         float v = row_value<KIND, 1>(a, x, o, at).v[0];
         if constexpr (KIND == kRowNorm) {
-            v = v * f * a.weight[at];
+            v = (float)(v * f) * a.weight[at];
             if (a.y) a.y[row * a.dim + at] = v;
         }
         top = max(top, mag(v));
@@ -256,7 +260,7 @@ __global__ __launch_bounds__(1024) void long_row_kernel(RowArgs a) {
             r.v[0] = a.y[row * a.dim + at];
         } else {
             r = row_value<KIND, 1>(a, x, o, at);
-            if constexpr (KIND == kRowNorm) r.v[0] = r.v[0] * f * a.weight[at];
+            if constexpr (KIND == kRowNorm) r.v[0] = (float)(r.v[0] * f) * a.weight[at];
         }
         store_codes<1>(a.codes + row * a.dim + at, r, inv);
     }

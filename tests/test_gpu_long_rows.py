@@ -43,3 +43,54 @@ def test_the_longest_row(torch_mod, gsp, ctx):
     assert torch.all(codes[dim:] == 77)
     del x, codes, w
     torch.cuda.empty_cache()
+
+
+def _rows64(x, w, eps):
+    """y in 64 bits on the device."""
+    d = x.double()
+    return d / (d.square().mean(-1, keepdim=True) + eps).sqrt() * w.double()
+
+
+@pytest.mark.parametrize("value", [None, 1.1, 0.3], ids=["random", "1.1", "0.3"])
+def test_sums_of_long_rows(torch_mod, ctx, value):
+    """A thread adds dim / 1024 squares; with equal values every addition can round the same way.
+
+    The squares, their sum and the root hold 64 bits, so y is off by its two roundings and the factor's: 3 steps."""
+    torch = torch_mod
+    rows, dim = 2, (1 << 24) + 3
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn((rows, dim), generator=g, device="cuda") if value is None else torch.full((rows, dim), value, device="cuda")
+    w = 1 + 0.2 * torch.randn(dim, generator=g, device="cuda")
+    y, codes = torch.zeros_like(x), torch.zeros((rows, dim), dtype=torch.uint8, device="cuda")
+    scale = torch.zeros(rows, device="cuda")
+    torch.cuda.synchronize()
+    ctx.rms_norm(rows, dim, x.data_ptr(), w.data_ptr(), 1e-5, y_ptr=y.data_ptr(), y_fp8_ptr=codes.data_ptr(),
+                 y_scale_ptr=scale.data_ptr())
+    ctx.sync()
+    want = _rows64(x, w, float(np.float32(1e-5)))
+    worst = ((y.double() - want).abs() / want.abs().clamp(min=1e-30)).max().item()
+    print(f"largest error {worst * 2 ** 24:.1f} steps", flush=True)
+    assert worst <= 3 * 2.0 ** -24
+    top = want.abs().amax(-1)
+    assert ((scale.double() - top / 448).abs() <= 5 * 2.0 ** -24 * top / 448).all()
+
+
+@pytest.mark.parametrize("dim", [32769, 40000])
+@pytest.mark.parametrize("eps", [0.0, 1e-6, 1e-42])
+def test_range_of_long_rows(torch_mod, ctx, dim, eps):
+    """Rows whose squares leave fp32: y is off by 3 steps, or a few of the least subnormals."""
+    torch = torch_mod
+    mags = [2.0 ** -140, 2.0 ** -100, 1e-24, 1e-19, 1.0, 2.0 ** 59, 2.0 ** 64, 2.0 ** 100, 2.0 ** 124]
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randn((len(mags), dim), generator=g, device="cuda").double() * torch.tensor(mags, dtype=torch.float64, device="cuda")[:, None]
+    x = x.float()
+    assert torch.isfinite(x).all()
+    w = 1 + 0.2 * torch.randn(dim, generator=g, device="cuda")
+    y = torch.zeros_like(x)
+    torch.cuda.synchronize()
+    ctx.rms_norm(len(mags), dim, x.data_ptr(), w.data_ptr(), eps, y_ptr=y.data_ptr())
+    ctx.sync()
+    want = _rows64(x, w, float(np.float32(eps)))
+    off = (y.double() - want).abs()
+    print([f"{(o / t.abs().clamp(min=1e-44)).max().item():.2g}" for o, t in zip(off, want)], flush=True)
+    assert (off <= 3 * 2.0 ** -24 * want.abs() + 4 * 2.0 ** -149).all()
