@@ -14,6 +14,8 @@
 // rows of 18944, gated, 4.5 us on the GPU, 2.2 TB/s (64 of 256 CUs).  A step's small
 // rows are bound by the launch: 8 rows of 896 take 2.8 us on the GPU, 64 of 3584
 // 3.8, and a call 3.4 us on the host.
+#include <cfloat>
+
 #include "gsp_internal.h"
 #include "../../include/glacier_paged.h"
 
@@ -22,6 +24,7 @@ namespace {
 
 constexpr float kE4m3Max = 448.0f;
 constexpr float kLeastTop = 0x1p-100f;  // the least largest magnitude a scale is taken from
+constexpr float kLeastMean = 0x1p-100f;  // of squares; the rounding of a subnormal one is 2^-150 at most
 constexpr int kRowMax = 32768;
 
 struct RowArgs {
@@ -147,6 +150,35 @@ __device__ inline Piece<VEC> row_value(const RowArgs& a, const float* x, const f
     return r;
 }
 
+// The mean of squares plus eps where squares leave fp32's range, with the row scaled by a power of two, which the norm's
+// factor undoes: the larger of the row's top and sqrt(eps) goes to 2^39 to 2^40.  32768 of its squares stay below 2^96,
+// and what is lost of small values' squares is far below them.  Rows of zeros, or with an infinity or a NaN, keep theirs.
+template <int VEC, int E>
+__device__ inline float scaled_mean(const RowArgs& a, Piece<VEC> (&r)[E], float* lsum, uint32_t* lmax) {
+    uint32_t top = 0;
+    float sq = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) top = max(top, mag(r[e].v[i]));
+    }
+    top = block_max(top, lmax);
+    int shift = 0;
+    if (top != 0 && top < 0x7f800000u) {
+        (void)frexpf(fmaxf(__uint_as_float(top), sqrtf(a.eps)), &shift);
+        shift = 40 - shift;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            r[e].v[i] = ldexpf(r[e].v[i], shift);
+            sq += r[e].v[i] * r[e].v[i];
+        }
+    }
+    return block_sum(sq, lsum) / (float)a.dim + ldexpf(a.eps, 2 * shift);
+}
+
 // One row in registers: E pieces of VEC values a thread.
 template <int KIND, int VEC, int E>
 __global__ __launch_bounds__(1024) void row_kernel(RowArgs a) {
@@ -186,7 +218,10 @@ __global__ __launch_bounds__(1024) void row_kernel(RowArgs a) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
             if (at0 + e * step < a.dim) w[e] = load_piece<VEC>(a.weight + at0 + e * step);
-        const float f = 1.0f / sqrtf(block_sum(sq, lsum) / (float)a.dim + a.eps);
+        float mean = block_sum(sq, lsum) / (float)a.dim + a.eps;
+        // Squares that fp32 does not hold: once more with the row scaled by a power of two.  Every thread has the same sum.
+        if (__builtin_expect(!(mean >= kLeastMean && mean <= FLT_MAX), 0)) mean = scaled_mean<VEC, E>(a, r, lsum, lmax);
+        const float f = 1.0f / sqrtf(mean);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int at = at0 + e * step;

@@ -284,9 +284,9 @@ int gsp_mrope_write_step(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, int32_t n_
  * fp32, which needs a residual; y_dev, y in fp32; y_fp8_dev with y_scale_dev,
  * y's codes and each row's scale max(max |y|, 2^-100) / 448, every code the
  * e4m3 value nearest to y / scale.  A row that holds a NaN gets NaN codes or a
- * NaN scale; one that holds an infinity gets a NaN or zero for every value, as
- * the formula does.  Squares and their sum are fp32: where they overflow (values
- * past 2^63) a row becomes 0.  sum_dev and y_dev may each be x_dev or residual_dev
+ * NaN scale; one whose s holds an infinity gets a NaN or zero for every value, as
+ * the formula does.  Finite rows of any magnitude keep their precision, also where
+ * squares leave fp32's range.  sum_dev and y_dev may each be x_dev or residual_dev
  * itself; every other overlap of an output with another argument is refused
  * (GSP_E_INVALID_ARG).  eps is finite and >= 0.  rows may be 0; dim is at least
  * 1.  Rows of any length and 4-byte alignment are taken; 16-byte aligned
