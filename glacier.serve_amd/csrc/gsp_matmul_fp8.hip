@@ -395,7 +395,7 @@ bool wide_loads(const MatmulFp8Args& a) { return a.in_dim % 256 == 0 && reinterp
 
 template <int WT, int MT, int R, int NT, int W>
 hipError_t launch_form(MatmulFp8Args a, hipStream_t stream) {
-    const int waves = even_waves((a.in_dim + 255) / 256, W);
+    const int waves = even_waves(a.in_dim / 256 + (a.in_dim % 256 != 0), W);  // in_dim may be close to 2^31
     const bool aligned = wide_loads(a);
     // A launch holds fewer than 2^32 threads: very large batches take several.
     const int64_t tiles = ((int64_t)a.out_dim + 16 * NT - 1) / (16 * NT);
