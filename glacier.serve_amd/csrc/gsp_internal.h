@@ -160,6 +160,7 @@ hipError_t launch_rope_write(int kv_f16, const RopeWriteArgs& a, hipStream_t str
 
 // Rotation by positions of several axes and Store (gsp_mrope.hip).
 constexpr int kMropeMaxAxes = 4;
+constexpr int64_t kMropeMaxItems = 65535 * 256;  // of a token: a launch's second grid dimension, 256 threads each
 struct MropeWriteArgs {
     void* k_pool;
     void* v_pool;

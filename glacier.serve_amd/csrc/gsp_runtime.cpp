@@ -998,6 +998,10 @@ int gsp_mrope_write_step(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, int32_t n_
         return gsp::fail(GSP_E_INVALID_ARG, "row strides (%lld, %lld, %lld) do not fit rows of %lld, %lld and %lld floats",
                          (long long)q_stride, (long long)k_stride, (long long)v_stride, (long long)wide,
                          (long long)wide_k, (long long)wide_v);
+    // A token's items, one pair or value each in the widest launch, are indexed with 32 bits and fit its grid.
+    if (((int64_t)n_heads + d.heads_kv) * (d.head_dim / 2) + wide_v > gsp::kMropeMaxItems)
+        return gsp::fail(GSP_E_UNSUPPORTED, "a token of %d and %d heads of %d is too wide for one launch", n_heads, d.heads_kv,
+                         d.head_dim);
     if (n == 0) return GSP_OK;
     if (!positions_dev || (n_heads > 0 && !q_out_dev)) return gsp::fail(GSP_E_INVALID_ARG, "positions/q_out is NULL");
     const auto span = [n](const void* p, int64_t stride, int64_t width) {

@@ -250,7 +250,8 @@ int gsp_rope_write_step_ex(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, int32_t 
  * fused projection can be given as they lie.  The turned Q goes to q_out_dev,
  * dense [total_q][n_heads][head_dim], which may be q_dev itself if that is
  * dense, and may not overlap any input otherwise (GSP_E_INVALID_ARG).  n_heads
- * 0 leaves Q out.  K and V go where gsp_rope_write_step stores them.  The tables
+ * 0 leaves Q out.  Tokens of more than 65535 * 256 pairs of Q and K and values of
+ * V are GSP_E_UNSUPPORTED.  K and V go where gsp_rope_write_step stores them.  The tables
  * travel with the launch: any may be used for the first time while the stream
  * captures.  Otherwise capture is as for gsp_rope_write_step. */
 #define GSP_MROPE_SECTIONS 0
