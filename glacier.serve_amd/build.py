@@ -31,6 +31,7 @@ SOURCES = [
     CSRC / "gsp_mrope.hip",
     CSRC / "gsp_noalloc.hip",
     CSRC / "gsp_runtime.cpp",
+    CSRC / "gsp_matmul_fp8_plan.cpp",
     CSRC / "gsp_step_plan.cpp",
     CSRC / "gsp_host_meta.cpp",
     CSRC / "gsp_status.cpp",

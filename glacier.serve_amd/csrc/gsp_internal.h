@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cstdint>
 
+#include "gsp_matmul_fp8_plan.h"
 #include "gsp_step_format.h"
 
 namespace gsp {
@@ -236,16 +237,6 @@ struct MatmulFp8Args {
     int32_t out_dim;
     int32_t batch;
 };
-// The kernel that a product takes, and the ranges of K that share an output (several only with a tile form).
-struct MatmulFp8Plan {
-    enum { kStream = 0, kWide, kTile64, kTile32 };
-    int32_t form = kStream;
-    int32_t splits = 1;
-    int32_t cus = 1;
-};
-// aligned: rows of weights are whole units of 256, 16-byte aligned.
-MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, bool aligned, int cus);
-int64_t matmul_fp8_x_bytes(int32_t in_dim, int32_t batch, const MatmulFp8Plan& plan);
 int64_t matmul_fp8_row_bytes(int32_t w_type, int32_t in_dim);
 hipError_t launch_matmul_fp8(int32_t w_type, const MatmulFp8Args& a, const MatmulFp8Plan& plan, hipStream_t stream);
 

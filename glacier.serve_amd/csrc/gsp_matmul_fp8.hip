@@ -23,7 +23,6 @@
 // operands agree, so lanes load long contiguous pieces (64 weights of a row,
 // 16 activations) and a 4 x 4 transposition among the four lanes of a column
 // (four register swaps, no LDS) deals every lane its dword of each piece.
-#include <cmath>
 #include <type_traits>
 
 #include "gsp_internal.h"
@@ -903,7 +902,7 @@ __global__ __launch_bounds__(64 * W) void matmul_fp8_stream32_kernel(MatmulFp8Ar
 // weights read before their unit begins, activations through registers, the barrier
 // behind a product, and 32 x 32 x 16 tiles of 64 or 32 rows (3584 x 3584 at 512 rows
 // 40 us instead of 32: too few waves a SIMD).
-constexpr int kWideRows = 128, kWideWaves = 8;
+constexpr int kWideRows = kMatmulFp8WideRows, kWideWaves = kMatmulFp8WideCols / 32;
 template <int WT, bool AL>
 __global__ __launch_bounds__(64 * kWideWaves) void matmul_fp8_wide_kernel(MatmulFp8Args a) {
     constexpr int kRow = Unit<WT>::kRow, kTile = 16 * kRow;
@@ -1202,17 +1201,10 @@ hipError_t launch_tile(const MatmulFp8Args& all, int splits, hipStream_t stream)
     });
 }
 
-// Converted activations of 32 rows take 16 KB a unit and 1 KB of sums.  A call keeps at most 1 GB of them: more rows
-// are multiplied piece by piece, each of many more workgroups than the chip holds.
-constexpr int64_t kConverted = 16384 + 1024;
-int64_t converted_rows(int units) {
-    return std::max<int64_t>(1, (1 << 30) / (units * kConverted) / (kWideRows / 32)) * kWideRows;
-}
-
 template <int WT>
 hipError_t launch_wide(const MatmulFp8Args& all, int splits, hipStream_t stream) {
     const int units = (all.in_dim + 255) / 256;
-    const int64_t most = std::min(converted_rows(units), launch_rows(units, kWideRows));
+    const int64_t most = std::min(matmul_fp8_converted_rows(units), launch_rows(units, kWideRows));
     return launch_tiles(all, splits, kWideRows, 32 * kWideWaves, most, stream, [&](MatmulFp8Args a, dim3 grid) {
         const int64_t tiles = ((int64_t)a.batch + kWideRows - 1) / kWideRows * (kWideRows / 32);
         a.sums = Unit<WT>::kMins ? a.xf + tiles * units * 16384 : nullptr;
@@ -1231,6 +1223,7 @@ hipError_t launch_type(const MatmulFp8Args& a, const MatmulFp8Plan& p, hipStream
         case MatmulFp8Plan::kWide: return launch_wide<WT>(a, p.splits, stream);
         case MatmulFp8Plan::kTile64: return launch_tile<WT, 4, 8>(a, p.splits, stream);
         case MatmulFp8Plan::kTile32: return launch_tile<WT, 2, 4>(a, p.splits, stream);
+        case MatmulFp8Plan::kStream32: return p.waves == 8 ? launch_stream32<WT, 8>(a, stream) : launch_stream32<WT, 4>(a, stream);
         default: break;
     }
     // The stream form.  With many outputs two tiles share a workgroup's activations; with few, more waves share a tile's
@@ -1243,16 +1236,7 @@ hipError_t launch_type(const MatmulFp8Args& a, const MatmulFp8Plan& p, hipStream
         return wide ? launch_form<WT, 1, 2, 2, 8>(a, stream) : launch_form<WT, 1, 2, 1, 16>(a, stream);
     if (a.batch <= 16)
         return wide ? launch_form<WT, 1, 4, 2, 8>(a, stream) : launch_form<WT, 1, 4, 1, 8>(a, stream);
-    // More rows, in 32 x 32 tiles where these fill more than half of the CUs: in one round with 8 waves each (3584 x 4608
-    // at 32 rows Q4_0 8.2 against 9.3, Q4_K 8.4 and 10.4; 3584 x 3584, on 112 CUs, 8.2 and 7.5), in several with 4, three
-    // a CU (Q4_0 4096 x 14336 at 32 rows 14.6 against 17.5, at 64 24.6 and 28.2), unless a second round would be short and
-    // much of the last rows' tile is empty (3584 x 4608 at 37 rows 14.1 and 11.3, 3584 x 8192 15.0 and 15.2).
-    const int64_t tiles = ((int64_t)a.out_dim + 31) / 32 * ((a.batch + 31) / 32);
-    if (a.batch <= 64 && wide_loads(a) && tiles > p.cus / 2) {
-        if (tiles <= p.cus) return launch_stream32<WT, 8>(a, stream);
-        if (a.batch <= 32 || a.batch > 48 || tiles >= 2 * p.cus) return launch_stream32<WT, 4>(a, stream);
-    }
-    // Otherwise 32 rows a workgroup while its workgroups, one a CU, run in one round (18944 x 3584 at 32 rows 18.9 us with
+    // More rows: 32 a workgroup while its workgroups, one a CU, run in one round (18944 x 3584 at 32 rows 18.9 us with
     // one tile); else 16 a workgroup (3584 x 4608 at 37 rows 11.3, 13 with 32).
     const int64_t tiles_b = (a.batch + 31) / 32;
     if (a.out_dim >= 16384 && a.batch <= 32) return launch_form<WT, 2, 4, 2, 4>(a, stream);
@@ -1262,63 +1246,6 @@ hipError_t launch_type(const MatmulFp8Args& a, const MatmulFp8Plan& p, hipStream
 }
 
 }  // namespace
-
-// Which form a product takes: the one whose modelled time is least.  A tile's
-// workgroup takes a time per unit of K that depends on how many share its CU;
-// workgroups run in rounds of what the chip holds; splits of K add the partial
-// sums' traffic and a launch.
-MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, bool aligned, int cus) {
-    MatmulFp8Plan best{};
-    best.cus = cus;
-    // Tile offsets are 32-bit; a longer K is streamed.  Up to 64 rows only wide outputs repay the conversion.
-    if (in_dim > (1 << 24) || batch <= (out_dim >= 16384 ? 32 : 64)) return best;
-    struct Form {
-        int form, rows, cols;
-        double us[4];   // a unit's time with one to four workgroups on a CU; 0: they do not fit
-        double around;  // a round's time before and behind its units
-    };
-    // Measured on 3584 and 18944 of K, Q4_0, at 65 to 2048 rows.
-    constexpr Form kForms[] = {{MatmulFp8Plan::kWide, kWideRows, 32 * kWideWaves, {4.3, 0, 0, 0}, 10},
-                               {MatmulFp8Plan::kTile64, 64, 128, {2.05, 3.7, 0, 0}, 4},
-                               {MatmulFp8Plan::kTile32, 32, 64, {1.33, 1.75, 2.5, 3.25}, 4}};
-    const int units = (in_dim + 255) / 256;
-    double least = 0;
-    if (batch <= 64 && aligned) {
-        // The stream's 32 x 32 tiles, three a CU: 3584 x 18944 at 48 rows 27.7 us against 31.9 in tiles of 64, 4096 x 32768
-        // 43.7 and 37.4, 1024 x 65536 33 and 20.
-        const double tiles = (double)(((int64_t)out_dim + 31) / 32 * ((batch + 31) / 32));
-        least = 7 + tiles / (3 * cus) * (1.2 + 0.86 * units);
-    }
-    for (const Form& f : kForms) {
-        if (batch <= f.rows / 2) continue;  // half of it empty: the next one takes less, and no workspace up to 64 rows
-        const double tiles = (double)(((int64_t)batch + f.rows - 1) / f.rows) * (((int64_t)out_dim + f.cols - 1) / f.cols);
-        int fit = 4;
-        while (fit > 1 && f.us[fit - 1] == 0) --fit;
-        for (int splits = 1; splits <= (batch > 64 ? 16 : 1) && splits * 2 <= std::max(2, units); ++splits) {
-            if (splits > 1 && tiles * splits > (double)cus * fit) break;
-            const int per = (units + splits - 1) / splits;
-            if ((units + per - 1) / per != splits) continue;
-            const double on_cu = std::ceil(tiles * splits / cus);
-            const double full = std::floor(on_cu / fit);
-            const int rest = (int)(on_cu - full * fit);
-            double t = (full * f.us[fit - 1] + (rest ? f.us[rest - 1] : 0)) * per;
-            t += f.around * (fit == 1 ? on_cu : 1);
-            if (splits > 1) t += 3.5 + (double)batch * out_dim * 4 * 2 * splits / 4e6;
-            if (least == 0 || t < least) {
-                least = t;
-                best.form = f.form;
-                best.splits = splits;
-            }
-        }
-    }
-    return best;
-}
-
-int64_t matmul_fp8_x_bytes(int32_t in_dim, int32_t batch, const MatmulFp8Plan& plan) {
-    if (plan.form != MatmulFp8Plan::kWide) return 0;
-    const int units = (in_dim + 255) / 256;
-    return (std::min<int64_t>(batch, converted_rows(units)) + kWideRows - 1) / kWideRows * (kWideRows / 32) * units * kConverted;
-}
 
 int64_t matmul_fp8_row_bytes(int32_t w_type, int32_t in_dim) {
     return (int64_t)(in_dim / 64) * (w_type == GSP_WTYPE_Q4_1 ? 40 : 36);
