@@ -4,6 +4,13 @@
 
 namespace gsp {
 
+// Converted activations of 32 rows take 16 KB a unit and 1 KB of sums.  A call keeps at most 1 GB of them: more rows
+// are multiplied piece by piece, each of many more workgroups than the chip holds.
+constexpr int64_t kConverted = 16384 + 1024;
+int64_t matmul_fp8_converted_rows(int units) {
+    return kMatmulFp8MostConverted / (units * kConverted) / (kMatmulFp8WideRows / 32) * kMatmulFp8WideRows;
+}
+
 // Which form a product takes: the one whose modelled time is least.  A tile's
 // workgroup takes a time per unit of K that depends on how many share its CU;
 // workgroups run in rounds of what the chip holds; splits of K add the partial
@@ -31,6 +38,8 @@ static MatmulFp8Plan least_time(int32_t in_dim, int32_t out_dim, int32_t batch, 
         least = 7 + tiles / (3 * cus) * (1.2 + 0.86 * units);
     }
     for (const Form& f : kForms) {
+        // K past 3.9 million: the activations of one workgroup's rows would not fit.
+        if (f.form == MatmulFp8Plan::kWide && matmul_fp8_converted_rows(units) == 0) continue;
         if (batch <= f.rows / 2) continue;  // half of it empty: the next one takes less, and no workspace up to 64 rows
         const double tiles = (double)(((int64_t)batch + f.rows - 1) / f.rows) * (((int64_t)out_dim + f.cols - 1) / f.cols);
         int fit = 4;
@@ -69,13 +78,6 @@ MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, bo
         if (plan.waves) plan.form = MatmulFp8Plan::kStream32;
     }
     return plan;
-}
-
-// Converted activations of 32 rows take 16 KB a unit and 1 KB of sums.  A call keeps at most 1 GB of them: more rows
-// are multiplied piece by piece, each of many more workgroups than the chip holds.
-constexpr int64_t kConverted = 16384 + 1024;
-int64_t matmul_fp8_converted_rows(int units) {
-    return std::max<int64_t>(1, (1 << 30) / (units * kConverted) / (kMatmulFp8WideRows / 32)) * kMatmulFp8WideRows;
 }
 
 int64_t matmul_fp8_x_bytes(int32_t in_dim, int32_t batch, const MatmulFp8Plan& plan) {

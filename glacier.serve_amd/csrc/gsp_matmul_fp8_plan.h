@@ -22,7 +22,9 @@ struct MatmulFp8Plan {
 // aligned: rows of weights are whole units of 256, 16-byte aligned.
 MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, bool aligned, int cus);
 
-// Workspace of the wide tile form: its converted activations.  Rows that a piece of the batch holds, and the bytes.
+// Workspace of the wide tile form, its converted activations: the most that a call keeps, the rows that a piece of the
+// batch holds (0: K too long for the form), and the bytes of a product.
+constexpr int64_t kMatmulFp8MostConverted = 1 << 30;
 int64_t matmul_fp8_converted_rows(int units);
 int64_t matmul_fp8_x_bytes(int32_t in_dim, int32_t batch, const MatmulFp8Plan& plan);
 

@@ -96,8 +96,9 @@ struct gsp_ctx {
     // ones.  A graph keeps the addresses it was captured with, so buffers of [1]
     // are never freed or replaced under it: one that must grow goes to `retired`
     // until gsp_shutdown, and each is at least twice the last, so the retired
-    // ones stay below the size of those in use.  Eager products never touch [1]:
-    // a replay on another stream runs beside them.
+    // ones stay below the size of those in use (activations double up to 1 GB only,
+    // what an 8-bit product keeps at most: below 2 GB).  Eager products never touch
+    // [1]: a replay on another stream runs beside them.
     MatmulBuffers mm[2];
     std::vector<void*> retired;
     hipEvent_t aux_done = nullptr;
@@ -253,6 +254,12 @@ int ensure_pinned(int32_t** buf, size_t* cap, size_t words, hipEvent_t done, boo
     return GSP_OK;
 }
 
+// The size that a buffer of `cap` elements takes when it has to hold `count`: at least twice the last, but up to
+// `most` elements no more than that.
+size_t grown(size_t cap, size_t count, size_t most) {
+    return std::max(count, count <= most ? std::min(cap * 2, most) : cap * 2);
+}
+
 // Grows a device buffer.  The stream is synchronised first so no queued
 // kernel still reads the old allocation.  A stream that is capturing into a
 // graph cannot do that: the call then fails with GSP_E_STATE, and the buffer
@@ -260,7 +267,7 @@ int ensure_pinned(int32_t** buf, size_t* cap, size_t words, hipEvent_t done, boo
 // workspace for every group up to 16).  `zero` clears the new buffer with a
 // kernel on the stream.
 template <typename T>
-int ensure_device(gsp_ctx* ctx, T** buf, size_t* cap, size_t count, bool zero) {
+int ensure_device(gsp_ctx* ctx, T** buf, size_t* cap, size_t count, bool zero, size_t most = 0) {
     if (count <= *cap) return GSP_OK;
     bool cap_on = false;
     int rc = is_capturing(ctx->stream, &cap_on);
@@ -272,7 +279,7 @@ int ensure_device(gsp_ctx* ctx, T** buf, size_t* cap, size_t count, bool zero) {
                          count * sizeof(T));
     rc = check_hip(hipStreamSynchronize(ctx->stream), "hipStreamSynchronize");
     if (rc) return rc;
-    size_t n = std::max(count, *cap * 2);
+    const size_t n = grown(*cap, count, most);
     if (*buf) (void)hipFree(*buf);
     *buf = nullptr;
     *cap = 0;
@@ -298,9 +305,9 @@ struct MatmulNeeds {
 // Grows a buffer of captured products while the stream captures.  The old one
 // is retired: nodes captured earlier hold its address.
 template <typename T>
-int grow_captured(gsp_ctx* ctx, T** buf, size_t* cap, size_t count) {
+int grow_captured(gsp_ctx* ctx, T** buf, size_t* cap, size_t count, size_t most = 0) {
     if (count <= *cap) return GSP_OK;
-    const size_t n = std::max(count, *cap * 2);
+    const size_t n = grown(*cap, count, most);
     // An allocation touches no stream; the relaxed mode lets it through a capture.
     hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
     int rc = check_hip(hipThreadExchangeStreamCaptureMode(&mode), "hipThreadExchangeStreamCaptureMode");
@@ -327,9 +334,11 @@ int matmul_workspace(gsp_ctx* ctx, const MatmulNeeds& need, bool cold_capture, M
     int rc = is_capturing(ctx->stream, &capturing);
     if (rc) return rc;
     *out = capturing ? &captured : &eager;
+    // Converted activations come close to the most that one call keeps: doubling past it would serve no call.
+    constexpr size_t most_x = gsp::kMatmulFp8MostConverted / sizeof(uint16_t);
     if (!capturing || !cold_capture) {
         rc = ensure_device(ctx, &eager.partials, &eager.partials_floats, need.partials, false);
-        if (!rc) rc = ensure_device(ctx, &eager.x, &eager.x_halves, need.x, false);
+        if (!rc) rc = ensure_device(ctx, &eager.x, &eager.x_halves, need.x, false, most_x);
         if (!rc) rc = ensure_device(ctx, &eager.exp, &eager.exp_words, need.exp, false);
         if (!rc) rc = ensure_device(ctx, &eager.sums, &eager.sums_floats, need.sums, false);
         if (!rc) rc = ensure_device(ctx, &eager.counters, &eager.counter_words, need.counters, true);
@@ -345,7 +354,7 @@ int matmul_workspace(gsp_ctx* ctx, const MatmulNeeds& need, bool cold_capture, M
         if (rc || !capturing) return rc;
     }
     rc = grow_captured(ctx, &captured.partials, &captured.partials_floats, need.partials);
-    if (!rc) rc = grow_captured(ctx, &captured.x, &captured.x_halves, need.x);
+    if (!rc) rc = grow_captured(ctx, &captured.x, &captured.x_halves, need.x, most_x);
     if (!rc) rc = grow_captured(ctx, &captured.exp, &captured.exp_words, need.exp);
     if (!rc) rc = grow_captured(ctx, &captured.sums, &captured.sums_floats, need.sums);
     return rc;

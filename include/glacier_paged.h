@@ -322,8 +322,9 @@ int gsp_quantize_fp8(gsp_ctx* ctx, int32_t act, int32_t rows, int32_t dim, int64
  * types).  Results are the same bit for bit on every call of the same sizes and
  * 16-byte alignment of W, captured or not; the number of rows and the alignment
  * may change the order of an output's sums.
- * Graph capture: products of more than 64 rows may need a workspace of up to about
- * 1 GB, so run the product itself once before capturing it (a larger one may take a
+ * Graph capture: products of more than 64 rows may need a workspace, of up to about
+ * 1 GB for a context's eager products and as much again for its captured ones, so run
+ * the product itself once before capturing it (a larger one may take a
  * form that needs none; GSP_E_STATE otherwise, and nothing is enqueued).  Captured
  * products keep buffers of their own, and their graphs must not run at the same time
  * as each other.  Up to 64 rows nothing is needed. */

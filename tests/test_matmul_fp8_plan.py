@@ -52,3 +52,13 @@ def test_ranges_cover_k(plan):
         assert ranges >= 1 and (ranges - 1) * per < units <= ranges * per
         assert (form == "stream32") == (waves > 0)
         assert ranges == 1 or b > 64  # a first call of up to 64 rows may be captured: no workspace
+
+
+def test_converted_activations_stay_within_a_gigabyte(plan):
+    """Whatever K is: where one workgroup's 128 rows alone would pass it, another form is taken."""
+    ks = [64, 3584, 18944, 131072, 1 << 20, 3947520, 3947584, 1 << 22, 1 << 23, (1 << 24) - 64, 1 << 24]
+    sizes = [(k, o, b) for k in ks for o in (64, 1000, 4096, 100000) for b in (65, 128, 129, 1024, 4097, 100000)]
+    got = plan(sizes, True)
+    assert max(g[4] for g in got) <= 1 << 30
+    assert all(g[4] == 0 and g[0] != "wide" for s, g in zip(sizes, got) if s[0] > 3947520)
+    assert any(g[0] == "wide" and g[4] > 1 << 29 for s, g in zip(sizes, got) if s[0] <= 3947520)
