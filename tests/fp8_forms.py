@@ -32,3 +32,5 @@ STREAMS = [
 ]
 # Weights of whole units at 16-byte addresses only.
 STREAM32 = [(256, 4500, 32, "stream32", 1, 1), (256, 8001, 64, "stream32", 1, 1)]
+# Ranges of K in a batch that goes piece by piece: 896 rows of converted activations at 2048 units.
+PIECES = [(524096, 250, 1600, "wide", 16, 128), (524288, 300, 1100, "wide", 14, 147)]

@@ -1,7 +1,9 @@
-"""What gsp_matmul_batch_fp8 keeps of device memory."""
+"""What gsp_matmul_batch_fp8 keeps of device memory, and batches that go piece by piece for it."""
+import numpy as np
 import pytest
 
-from fp8_helpers import Q4_1
+from fp8_forms import PIECES
+from fp8_helpers import E4M3, Q4_0, Q4_1, Q4_K, decode_weights, random_weights
 
 pytestmark = pytest.mark.gpu
 
@@ -26,4 +28,39 @@ def test_converted_activations_do_not_double_past_a_gigabyte(torch_mod, gsp):
     assert 0.9e9 < kept[0] <= 1.0e9 and 1.0e9 < kept[1] <= 1.15e9
     ctx.close()
     del x, w
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("w_type", [Q4_0, Q4_1, Q4_K], ids=["q4_0", "q4_1", "q4_k"])
+@pytest.mark.parametrize("case", PIECES, ids=lambda c: f"in{c[0]}_out{c[1]}_b{c[2]}")
+def test_pieces_of_a_batch_with_ranges_of_k(torch_mod, ctx, case, w_type):
+    """Every piece adds up its own ranges.  The weights are eight rows over and over, so that every output has its 64 bits."""
+    torch = torch_mod
+    in_dim, out_dim, batch, _, ranges, _ = case
+    if w_type == Q4_K and in_dim % 256:
+        pytest.skip("K-quants have K in units of 256")
+    print(f"case pieces {w_type} {case}", flush=True)
+    rng = np.random.default_rng(out_dim)
+    eight = random_weights(rng, w_type, 8, in_dim)
+    which = torch.from_numpy(rng.integers(0, 8, out_dim)).cuda()
+    w = torch.from_numpy(eight).cuda()[which]
+    x = torch.randint(0, 254, (batch, in_dim), dtype=torch.uint8, device="cuda")
+    x[x == 0x7f] = 0xfe  # every code but NaN
+    s = torch.rand(batch, device="cuda") + 0.5
+    y = torch.full((64 + batch * out_dim + 64,), 77.0, device="cuda")
+    torch.cuda.synchronize()
+    ctx.matmul_batch_fp8(w_type, w.data_ptr(), x.data_ptr(), s.data_ptr(), y[64:].data_ptr(), in_dim, out_dim, batch)
+    ctx.sync()
+    assert torch.all(y[:64] == 77) and torch.all(y[-64:] == 77)
+    wm, mag = (torch.from_numpy(a.T.copy()).cuda() for a in decode_weights(w_type, eight, in_dim))
+    table = torch.from_numpy(E4M3).cuda()
+    got = y[64:-64].view(batch, out_dim)
+    for at in range(0, batch, 200):
+        part = table[x[at: at + 200].int()] * s[at: at + 200, None].double()
+        want, bound = (part @ wm)[:, which], (37 + in_dim / 16 + ranges) * 2.0 ** -23 * (part.abs() @ mag)[:, which]
+        err = (got[at: at + 200].double() - want).abs()
+        assert (err <= bound).all(), at
+        # the bound grows with K's length, the error of sums in any order hardly: a lost range would be a large part
+        assert (err <= 1e-4 * (part.abs() @ mag)[:, which]).all(), at
+    del x, y
     torch.cuda.empty_cache()

@@ -4,7 +4,7 @@ from pathlib import Path
 
 import pytest
 
-from fp8_forms import CUS, STREAM32, STREAMS, TILES
+from fp8_forms import CUS, PIECES, STREAM32, STREAMS, TILES
 
 NATIVE = Path(__file__).resolve().parent / "native"
 
@@ -26,7 +26,7 @@ def plan():
 
 @pytest.mark.parametrize("aligned", [True, False])
 def test_sizes_reach_their_forms(plan, aligned):
-    cases = TILES + (STREAM32 if aligned else STREAMS)
+    cases = TILES + PIECES + (STREAM32 if aligned else STREAMS)
     got = plan([c[:3] for c in cases], aligned)
     assert [(c, g[:3]) for c, g in zip(cases, got) if g[:3] != c[3:]] == []
 
@@ -62,3 +62,8 @@ def test_converted_activations_stay_within_a_gigabyte(plan):
     assert max(g[4] for g in got) <= 1 << 30
     assert all(g[4] == 0 and g[0] != "wide" for s, g in zip(sizes, got) if s[0] > 3947520)
     assert any(g[0] == "wide" and g[4] > 1 << 29 for s, g in zip(sizes, got) if s[0] <= 3947520)
+
+
+def test_pieces_are_pieces(plan):
+    for (k, _, batch, *_), got in zip(PIECES, plan([c[:3] for c in PIECES], True)):
+        assert got[4] == 896 // 32 * 2048 * (16384 + 1024) and batch > 896
