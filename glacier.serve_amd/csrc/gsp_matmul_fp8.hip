@@ -437,8 +437,9 @@ __device__ inline void lds_barrier() {
 // group's weights are expanded.  Q4_K's scales are integers within the operand, so that
 // its sums run over the eight groups of a super-block in the matrix unit alone.
 // Minimums meet the sums of x in one more product a unit: staging adds up each group,
-// and leaves its sum as two fp16 numbers, the nearest and what that leaves (22 bits; a
-// sum has up to 23).
+// and leaves its sum as two fp16 numbers, the nearest and what that leaves, which hold
+// every such sum: it is a multiple of 2^-9 below 2^14, and the rest, of either sign, at
+// most half a step of the nearest.
 //
 // Two heights: 64 rows by 128 (Q4_0, 3584 x 3584 at 512 rows 31.6 us, 416 TFLOP/s) and
 // 32 by 64 where that fills the chip better (896 x 4864 at 65 rows 7.8 us).
@@ -763,7 +764,7 @@ __device__ inline f16v mfma32(const Terms& a, const Terms& b, f16v c) {
 // they are.  A unit's sums of x by group are products as well, with ones in row g for
 // group g: they arrive as [group][batch row], four groups a lane half, and meet the
 // minimums as two fp16 numbers each in one product.  Rows of weights are whole units,
-// 16-byte aligned.  us, 64 rows of 18944 x 3584: Q4_0 23.3, Q4_1 25.5, Q4_K 24.9, with
+// 16-byte aligned.  us, 64 rows of 18944 x 3584: Q4_0 22.9, Q4_1 24.1, Q4_K 24.5, with
 // 16 x 16 x 32 products 26.7, 33.3 and 31.9: fewer of them, no swaps of activations, and
 // minimums and Q4_K's scales without the vector unit, whose issue bounds both.
 template <int WT, int W>
@@ -891,12 +892,17 @@ __global__ __launch_bounds__(64 * W) void matmul_fp8_stream32_kernel(MatmulFp8Ar
 // The wide tile form: 128 batch rows by 256 weight rows a workgroup, 128 by 32 a wave,
 // in the 32 x 32 x 16 instruction, of which half as many are issued for the same terms.
 // Beside a multiply-add for each output it takes 9.3 ns a SIMD for 16 x 16 x 32 terms,
-// the other one 11.2, and issue is what bounds this form: the vector unit is busy 73 %
-// of the time (Q4_0, 3584 x 18944 at 2048 rows), with 512 multiply-adds, 176
-// instructions of expansion, 64 products and 63 others a wave and unit; the matrix unit
-// 43 %.  Activations come converted from matmul_fp8_convert_kernel (9 us there), as
-// converting them in every workgroup took 4 % longer.  us at 2048 rows (TFLOP/s), 3584 x
-// 18944 and 18944 x 3584: Q4_0 319 (872) and 307, Q4_1 317 and 310, Q4_K 310 and 298.
+// the other one 11.2.  With Q4_0 and Q4_1 the vector unit issues three quarters of the
+// time (3584 x 18944 at 2048 rows), with 512 multiply-adds, 176 instructions of expansion
+// (Q4_0), 64 products and 63 others a wave and unit; the matrix unit is busy 45 %.  Q4_K,
+// whose scales are in its operands, has 35 % fewer instructions and takes 3 % less: both
+// units are busy half of the time, and waves wait to issue a third of it.  LDS leaves room
+// for one workgroup a CU, two waves a SIMD to cover each other's products.  Activations
+// come converted from matmul_fp8_convert_kernel (9 us there), as converting them in every
+// workgroup took 4 % longer.  us at 2048 rows (TFLOP/s), 3584 x 18944 and 18944 x 3584:
+// Q4_0 331 (840) and 326, Q4_1 338 and 330, Q4_K 324 and 315; another card took 4 % less.
+// Q4_1 with 4-byte loads is short of registers and spills 13 of them (896 x 9728 at 2048
+// rows 92 us, Q4_0 78).
 //
 // Measured without gain: the loads to LDS sent one by one between the products, the
 // weights read before their unit begins, activations through registers, the barrier
@@ -1164,7 +1170,7 @@ hipError_t launch_stream32(const MatmulFp8Args& a, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// Rows of a launch, which holds fewer than 2^32 threads: very large batches take several (and no splits).
+// Rows of a launch, which holds fewer than 2^32 threads: very large batches take several.
 int64_t launch_rows(int64_t others, int rows) { return std::max<int64_t>(1, (1 << 21) / others) * rows; }
 
 void add_splits(const MatmulFp8Args& a, int splits, hipStream_t stream) {

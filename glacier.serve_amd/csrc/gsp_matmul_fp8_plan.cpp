@@ -32,7 +32,8 @@ static MatmulFp8Plan least_time(int32_t in_dim, int32_t out_dim, int32_t batch, 
     const int units = (in_dim + 255) / 256;
     double least = 0;
     if (batch <= 64 && aligned) {
-        // The stream's 32 x 32 tiles, three a CU: 3584 x 18944 at 48 rows 27.7 us against 31.9 in tiles of 64, 4096 x 32768
+        // The stream's 32 x 32 tiles, three a CU with Q4_0, whose times stand for all three types (registers leave two of
+        // Q4_1's and Q4_K's: 3584 x 18944 at 64 rows 28.3, 31.2 and 29.5 us): 3584 x 18944 at 48 rows 27.7 us against 31.9 in tiles of 64, 4096 x 32768
         // 43.7 and 37.4, 1024 x 65536 33 and 20.
         const double tiles = (double)(((int64_t)out_dim + 31) / 32 * ((batch + 31) / 32));
         least = 7 + tiles / (3 * cus) * (1.2 + 0.86 * units);
@@ -69,7 +70,7 @@ MatmulFp8Plan plan_matmul_fp8(int32_t in_dim, int32_t out_dim, int32_t batch, bo
     if (plan.form != MatmulFp8Plan::kStream) return plan;
     // Streamed products of 17 to 64 rows, in 32 x 32 tiles where these fill more than half of the CUs: in one round with 8
     // waves each (3584 x 4608 at 32 rows Q4_0 8.2 against 9.3, Q4_K 8.4 and 10.4; 3584 x 3584, on 112 CUs, 8.2 and 7.5),
-    // in several with 4, three a CU (Q4_0 4096 x 14336 at 32 rows 14.6 against 17.5, at 64 24.6 and 28.2), unless a second
+    // in several with 4, three a CU (Q4_1 and Q4_K two; Q4_0 4096 x 14336 at 32 rows 14.6 against 17.5, at 64 24.6 and 28.2), unless a second
     // round would be short and much of the last rows' tile is empty (3584 x 4608 at 37 rows 14.1 and 11.3, 3584 x 8192
     // 15.0 and 15.2).
     const int64_t tiles = ((int64_t)out_dim + 31) / 32 * ((batch + 31) / 32);

@@ -3,8 +3,9 @@
 // K and V read once and written into their slots.  The angles' rates come with
 // the launch's arguments (made on the host, 64 powers in fp64 that would else
 // cost every workgroup a third of its time), so that no table has to be on the device.
-// Sixteen prompts, 7700 tokens of 28 + 4 heads of 128, take 54 us, 5.3 TB/s; a decode
-// step of 64 rows is bound by the launch.
+// Sixteen prompts, 7700 tokens of 28 + 4 heads of 128, take 58.6 us with other buffers
+// than the call before, 4.8 TB/s as a large copy, and 51 where part of them is still in
+// the last-level cache; a decode step of 64 rows is bound by the launch.
 #include "gsp_internal.h"
 #include "gsp_rope.h"
 #include "../../include/glacier_paged.h"
@@ -138,7 +139,8 @@ template <typename KT, int VEC>
 void launch_form(const MropeWriteArgs& a, hipStream_t stream) {
     const int items = (a.n_heads + a.n_kv) * (a.head_dim / (2 * VEC)) + a.n_kv * (a.v_head_dim / VEC);
     // One item a thread spreads a decode tick over more workgroups; with many tokens three let a workgroup share its
-    // angles among more loads (7966 tokens of 28/4 heads, d 128, fp32 pages: 57.6 us with one, 53.9 with three, 5.3 TB/s).
+    // angles among more loads (7966 tokens of 28/4 heads, d 128, fp32 pages: 57.6 us with one, 53.9 with three, launches
+    // of two streams overlapping).
     constexpr int kMany = 3;
     if (a.n < 512)
         hipLaunchKernelGGL((mrope_write_kernel<KT, VEC, 1>), dim3(a.n, (items + 255) / 256), dim3(256), 0, stream, a);

@@ -6,14 +6,18 @@
 // One workgroup takes one row and holds it in registers: every input is read
 // once and every output written once, with the row's two reductions (the sum
 // of squares, then the largest magnitude) between.  Rows past what a
-// workgroup's registers hold (kRowMax values) are read again for each pass.
+// workgroup's registers hold (kRowMax values) are read again for each pass, a
+// value at a time.
 //
 // Bound by memory where there is enough of it: 8193 rows of 4096 with a residual
-// and all three results 112 us, 5.1 TB/s (a large copy reaches 4.8); 4099 rows of
-// 3584 into codes 11.8 us, 6.2 TB/s (the inputs lie in the last-level cache); 64
-// rows of 18944, gated, 4.5 us on the GPU, 2.2 TB/s (64 of 256 CUs).  A step's small
-// rows are bound by the launch: 8 rows of 896 take 2.8 us on the GPU, 64 of 3584
-// 3.8, and a call 3.4 us on the host.
+// and all three results 112 us, 5.1 TB/s (a large copy reaches 4.8); 4096 gated rows
+// of 18944 135 us, 5.2 TB/s; 4099 rows of 3584 into codes 11.8 us, 6.2 TB/s (the
+// inputs lie in the last-level cache); 64 gated rows of 18944 5.0 us, 2.2 TB/s (64 of
+// 256 CUs).  A step's small rows are bound by the launch: 8 rows of 896 take 2.8 us on
+// the GPU, 64 of 3584 3.8, and a call 3.4 us on the host.  At 4-byte addresses or of
+// odd lengths the first take 132 us and the codes of 4099 rows 17.6.  Long rows
+// occupy one workgroup each: 4096 of 40000 with all results 919 us (3.0 TB/s), codes
+// alone 317 (2.6); 64 of them 54 and 16.
 #include <cfloat>
 
 #include "gsp_internal.h"
@@ -126,8 +130,8 @@ __device__ inline void store_codes(uint8_t* p, const Piece<VEC>& r, float inv) {
 
 // g / (1 + exp(-g)) * u.  exp(-g) is 2^t with t = -g log2(e) rounded, times 1 + ln 2 times what the rounding left,
 // which keeps the hardware's 2^t (one step) that exact for every t; the quotient is a product with the hardware's
-// reciprocal (one step).  In all four steps, at 12 instructions; with expf and the division the kernel spent
-// more time on them than on memory (64 rows of 18944: 6.7 us against 5.8).  Past +-200 the exponential is 0 or
+// reciprocal (one step).  In all four steps, at 12 instructions; with expf and the division the kernel spends
+// more time on them than on memory (64 rows of 18944: 6.7 us against 5.2).  Past +-200 the exponential is 0 or
 // infinity in fp32 anyway, and the clamp keeps infinities out of the remainder.
 __device__ inline float silu_mul(float g, float u) {
     constexpr float kL = 1.44269502f, kLLow = 1.92596299e-8f, kLn2 = 0.693147182f;  // log2(e) in two parts

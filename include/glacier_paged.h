@@ -284,14 +284,16 @@ int gsp_mrope_write_step(gsp_ctx* ctx, gsp_pool* pool, int32_t layer, int32_t n_
  * Results, each left out with NULL (one at least is asked for): sum_dev, s in
  * fp32, which needs a residual; y_dev, y in fp32; y_fp8_dev with y_scale_dev,
  * y's codes and each row's scale max(max |y|, 2^-100) / 448, every code the
- * e4m3 value nearest to y / scale.  A row that holds a NaN gets NaN codes or a
- * NaN scale; one whose s holds an infinity gets a NaN or zero for every value, as
- * the formula does.  Finite rows of any magnitude keep their precision, also where
- * squares leave fp32's range.  sum_dev and y_dev may each be x_dev or residual_dev
- * itself; every other overlap of an output with another argument is refused
- * (GSP_E_INVALID_ARG).  eps is finite and >= 0.  rows may be 0; dim is at least
+ * e4m3 value nearest to y / scale (where that lies within 3 * 2^-24 of itself from
+ * the middle between two codes, either of them).  A row that holds a NaN gets NaN
+ * codes or a NaN scale; one whose s holds an infinity gets a NaN or zero for every
+ * value, as the formula does.  Finite rows of any magnitude keep their precision,
+ * also where squares leave fp32's range.  sum_dev and y_dev may each be x_dev or
+ * residual_dev itself; every other overlap of an output with another argument is
+ * refused (GSP_E_INVALID_ARG).  eps is finite and >= 0.  rows may be 0; dim is at least
  * 1.  Rows of any length and 4-byte alignment are taken; 16-byte aligned
- * buffers with dim a multiple of 4 are read and written 16 bytes at a time. */
+ * buffers with dim a multiple of 4, up to 32768, are read and written 16 bytes at
+ * a time, and longer rows are read once for each pass over them. */
 int gsp_rms_norm(gsp_ctx* ctx, int32_t rows, int32_t dim, const float* x_dev, const float* residual_dev,
                  const float* weight_dev, float eps, float* sum_dev, float* y_dev, uint8_t* y_fp8_dev,
                  float* y_scale_dev);
@@ -316,8 +318,9 @@ int gsp_quantize_fp8(gsp_ctx* ctx, int32_t act, int32_t rows, int32_t dim, int64
  * (GSP_WTYPE_Q4_0, 18 bytes: fp16 d, then 16 bytes whose low halves are weights
  * 0 to 15 and whose high halves are 16 to 31, w = d * (q - 8)) and Q4_1
  * (GSP_WTYPE_Q4_1, 20 bytes: fp16 d, fp16 m, the same 16 bytes, w = d * q + m).
- * Products of codes and quants are exact and sums are fp32: no rounding of x or
- * W is added to the codes' own.  in_dim is a multiple of 64 (256 for Q4_K)
+ * Products of codes and quants are exact, sums of x that a minimum multiplies are
+ * held whole (as fp16 pairs in the forms of many rows) and all other sums are fp32: no
+ * rounding of x or W is added to the codes' own.  in_dim is a multiple of 64 (256 for Q4_K)
  * and out_dim at most 2^24 (GSP_E_UNSUPPORTED otherwise, as for other weight
  * types).  Results are the same bit for bit on every call of the same sizes and
  * 16-byte alignment of W, captured or not; the number of rows and the alignment
